@@ -27,11 +27,15 @@ SOURCES = [
     "kernels/rmsnorm.cu",
     "kernels/comm_kernels.cu",
     "kernels/no_alloc_entry.cu",
+    "kernels/kv_cache.cu",
+    "kernels/paged_attention.cu",
+    "kernels/prompt_attention.cu",
     "runtime/symm_heap.cpp",
     "runtime/engine.cpp",
     "api/nccl_utils.cpp",
     "api/overlap_impl.cpp",
     "api/baseline_impl.cpp",
+    "api/attention_ops.cpp",
     "api/bindings.cpp",
 ]
 

@@ -1,4 +1,10 @@
 """Functional wrappers over the native operators."""
+from .attention import (  # noqa: F401
+    cache_append,
+    copy_pages,
+    paged_attention,
+    prompt_attention,
+)
 from .functional import (  # noqa: F401
     a2a_dispatch_gemm,
     allgather_gemm,
