@@ -1,6 +1,26 @@
 // Attention of a prompt: causal, with an optional window of recent tokens and first tokens that stay visible.
+//
+// A CTA takes two tiles of 128 rows of one key and value head; a row is a token and one of the query heads that share the
+// head, so that a tile of grouped heads spans few tokens and little of it is hidden by the diagonal.  For every tile of 128
+// visible tokens, scores S = Q K^T go from the tensor cores into TMEM, a thread per row turns its 128 scores into weights,
+// P goes back into TMEM over S, and O += P V accumulates there.  While the tensor cores work for one tile of rows, 128 threads
+// compute the weights of the other.
+//
+//   warps 0-3, 4-7   softmax of the two tiles: warp w reads the TMEM lanes 32 (w % 4) .. + 31, a thread is a row
+//   warp 8           TMA: Q once, then K and V tile by tile into a ring of buffers
+//   warp 9           tcgen05.mma: S_i = Q_i K_j^T from shared memory, O_i += P_i V_j with P_i in TMEM
+//   warps 10, 11     none (registers are handed over by four warps at a time)
+//
+// TMEM (512 columns of 32 bits): S_0, S_1 (128 each; P_i, 16-bit pairs, over the first 64 of S_i), O_0, O_1 (head_dim each).
+//
+// The running largest score of a row only moves when it grows by more than 8 (in powers of two): until then weights are up
+// to 2^8 instead of 1, which costs no accuracy (P is a floating-point type, sums are fp32), and O is not rescaled.
 #include <algorithm>
 #include <cmath>
+#include <cstring>
+
+#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include "attention_common.cuh"
 
@@ -65,19 +85,527 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const __grid_constant_
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kTileRows = 128, kTileKeys = 128;
+constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
+constexpr uint64_t kDeadlineNs = 4000000000ull;  // of a wait; nothing here takes a thousandth of it
+constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
+
+template <int D>
+constexpr int ring_buffers() {
+  return D == 128 ? 5 : 8;
+}
+template <int D>
+constexpr int key_tile_bytes() {
+  return kTileKeys * D * 2;
+}
+// shared memory behind the first 1024-byte boundary: two Q tiles, then the ring
+template <int D>
+constexpr int prompt_smem_bytes() {
+  return 2 * kTileRows * D * 2 + ring_buffers<D>() * key_tile_bytes<D>() + 1024;
+}
+
+struct PromptArgs {
+  PromptParams p;
+  CUtensorMap q, k, v;
+  int group, tokens;         // query heads of a head, tokens of a tile
+  int blocks, q_batch, k_batch, v_batch, k_head, v_head, q_head;  // pairs of tiles; 0 where a dimension is broadcast, else 1
+  float scale_log2;
+};
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(ptx::smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+      : "memory");
+}
+// B as stored by a TMA load of [tokens][64 values] boxes, 128-byte swizzle, read along the tokens (MN-major): groups of 8
+// tokens are 1024 bytes apart, the next 64 columns `block_bytes`.
+__device__ __forceinline__ uint64_t make_smem_desc_mn_sw128(uint32_t smem_addr, uint32_t block_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
+  d |= static_cast<uint64_t>(block_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+// D[TMEM] (+)= A[TMEM] B[shared memory]
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bits lo .. hi (inclusive) of a 32-bit word; none if hi < lo.
+__device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
+  lo = max(lo, 0);
+  hi = min(hi, 31);
+  return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
+}
+template <bool BF16>
+__device__ __forceinline__ bool pair_not_finite(uint32_t u) {
+  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
+  return (u & e) == e || (u & (e << 16)) == (e << 16);
+}
+
+// What a CTA works on.
+struct PromptBlock {
+  int b, kv_head, t0, length;  // first token of the first tile
+  SeenTiles tiles;
+  int n;  // tiles of keys; 0: no row sees anything
+};
+
 template <int D, bool BF16>
-cudaError_t launch_typed(const PromptParams& p, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.batch) * p.sq * p.heads;
-  const long long grid = std::min<long long>((rows + 7) / 8, 8ll * device_sm_count());
-  return launch_after(prompt_rows_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p);
+__global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int NB = ring_buffers<D>(), TILE = key_tile_bytes<D>(), BLOCK = kTileKeys * 128;
+  const PromptParams& p = a.p;
+  extern __shared__ __align__(128) uint8_t raw[];
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[NB], kv_empty[NB], s_full[2], p_full[2], o_done[2], v_ok;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed, dirty;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t smem = (ptx::smem_u32(raw) + 1023u) & ~1023u;
+  const uint32_t ring = smem + 2 * kTileRows * D * 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_full[i], kTileRows);
+      ptx::mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      ptx::mbar_init(&kv_full[i], 1);
+      ptx::mbar_init(&kv_empty[i], 1);
+    }
+    ptx::mbar_init(&v_ok, kSoftmaxThreads);
+    ptx::mbar_fence_init();
+    ptx::fence_proxy_async_smem();
+    failed = 0;
+    dirty = 0;
+  }
+  if (warp == 8) {
+    if (lane == 0) {
+      ptx::prefetch_tensormap(&a.q);
+      ptx::prefetch_tensormap(&a.k);
+      ptx::prefetch_tensormap(&a.v);
+    }
+    __syncwarp();
+    ptx::tmem_alloc(&tmem_slot, 512);
+    ptx::tmem_relinquish();
+    ptx::tc_fence_before_sync();
+  }
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  ptx::wait_for_previous_kernel();
+
+  PromptBlock blk;
+  {
+    // late tokens first: they see the most keys
+    const int per = p.batch * p.kv_heads;
+    const int qb = blockIdx.x / per, rest = blockIdx.x - qb * per;
+    blk.b = rest / p.kv_heads;
+    blk.kv_head = rest - blk.b * p.kv_heads;
+    blk.t0 = (a.blocks - 1 - qb) * 2 * a.tokens;
+    blk.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + blk.b), 0), p.sk);
+    const int p0 = p.sk - p.sq + blk.t0, p1 = p.sk - p.sq + min(blk.t0 + 2 * a.tokens, p.sq) - 1;
+    blk.tiles = seen_tiles(p0, p1, blk.length, p.window, p.sinks, kTileKeys);
+    blk.n = p0 < blk.length ? blk.tiles.count() : 0;
+  }
+  // Whether every row of tile i (0, 1) sees all of a tile of keys; if not, scores are masked and the values are looked at.
+  auto whole = [&](int i, int first_key) {
+    const int lo = p.sk - p.sq + blk.t0 + i * a.tokens, hi = min(lo + a.tokens, p.sk) - 1, last_key = first_key + kTileKeys - 1;
+    return last_key <= lo && last_key < blk.length && hi < blk.length &&
+           (p.window == 0 || hi - first_key < p.window || last_key < p.sinks);
+  };
+  const uint64_t deadline = ptx::globaltimer_ns() + kDeadlineNs;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ptx::mbar_wait(bar, parity, deadline)) return true;
+    failed = 1;
+    return false;
+  };
+  // the lanes of a warp go on, or give up, together
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+  // 384 threads x 168 registers at launch = 128 x 56 + 256 x 224
+  auto hand_over = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); };
+  if (warp == 8) {
+    hand_over();
+    if (lane == 0 && blk.n > 0) {
+      const int rows = a.group * a.tokens;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_arrive_expect_tx(&q_full[i], rows * D * 2);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) {
+          tma_load_4d(smem + (i * (D / 64) + c) * (kTileRows * 128), &a.q, &q_full[i], c * 64,
+                      blk.kv_head * a.group * a.q_head, blk.t0 + i * a.tokens, blk.b * a.q_batch);
+        }
+      }
+      int buf = 0;
+      uint32_t round = 0;
+      for (int j = 0; j < blk.n; ++j) {
+        const int key = blk.tiles.tile(j) * kTileKeys;
+        bool ok = true;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (round > 0) ok = ok && wait(&kv_empty[buf], (round - 1) & 1u);
+          if (!ok) break;
+          ptx::mbar_arrive_expect_tx(&kv_full[buf], TILE);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c) {
+            tma_load_4d(ring + buf * TILE + c * BLOCK, kv == 0 ? &a.k : &a.v, &kv_full[buf], c * 64, key,
+                        blk.kv_head * (kv == 0 ? a.k_head : a.v_head), blk.b * (kv == 0 ? a.k_batch : a.v_batch));
+          }
+          if (++buf == NB) {
+            buf = 0;
+            ++round;
+          }
+        }
+        if (!ok) break;
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    hand_over();
+    if (lane == 0 && blk.n > 0) {
+      constexpr int FMT = BF16 ? 1 : 0;
+      constexpr uint32_t idesc_s = ptx::make_idesc_f16(FMT, kTileRows, kTileKeys);
+      constexpr uint32_t idesc_o = ptx::make_idesc_f16(FMT, kTileRows, D) | (1u << 16);  // B along its rows
+      auto scores = [&](int i, uint32_t keys) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * BLOCK + (k & 3) * 32;
+          ptx::umma_f16_ss(tmem + i * kTileKeys,
+                           ptx::make_smem_desc_k_sw128(smem + i * (D / 64) * (kTileRows * 128) + off),
+                           ptx::make_smem_desc_k_sw128(keys + off), idesc_s, k > 0);
+        }
+        ptx::umma_commit(&s_full[i]);
+      };
+      auto outputs = [&](int i, uint32_t values, bool first) {
+#pragma unroll
+        for (int k = 0; k < kTileKeys / 16; ++k) {
+          umma_f16_ts(tmem + 2 * kTileKeys + i * 128, tmem + i * kTileKeys + k * 8,
+                      make_smem_desc_mn_sw128(values + k * 16 * 128, BLOCK), idesc_o, !first || k > 0);
+        }
+        ptx::umma_commit(&o_done[i]);
+      };
+      int buf = 0;
+      uint32_t round = 0, guards = 0;
+      auto next = [&] {
+        if (++buf == NB) {
+          buf = 0;
+          ++round;
+        }
+      };
+      bool ok = true;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        ok = ok && wait(&q_full[i], 0);
+        if (i == 0) ok = ok && wait(&kv_full[0], 0);
+        if (ok) scores(i, ring);
+      }
+      if (ok) ptx::umma_commit(&kv_empty[0]);
+      next();
+      for (int j = 0; ok && j < blk.n; ++j) {
+        const int first_key = blk.tiles.tile(j) * kTileKeys;
+        const int vbuf = buf;
+        ok = wait(&kv_full[vbuf], round & 1u);
+        next();
+        const int kbuf = buf;
+        const bool more = j + 1 < blk.n;
+        if (ok && more) {
+          ok = wait(&kv_full[kbuf], round & 1u);
+          next();
+        }
+        if (ok && !(whole(0, first_key) && whole(1, first_key))) {
+          ok = wait(&v_ok, guards & 1u);
+          ++guards;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ok = ok && wait(&p_full[i], j & 1u);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          outputs(i, ring + vbuf * TILE, j == 0);
+          if (i == 1) ptx::umma_commit(&kv_empty[vbuf]);
+          if (more) {
+            scores(i, ring + kbuf * TILE);
+            if (i == 1) ptx::umma_commit(&kv_empty[kbuf]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    hand_over();
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int tile = warp >> 2;
+    const int row = threadIdx.x & 127;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes each, in the upper half of an address
+    const uint32_t t_s = tmem + lanes + tile * kTileKeys, t_o = tmem + lanes + 2 * kTileKeys + tile * 128;
+    const int token = row / a.group, head = row - token * a.group;
+    const int t = blk.t0 + tile * a.tokens + token;
+    const int pos = p.sk - p.sq + t;
+    const bool real = token < a.tokens && t < p.sq;
+    const int last = real && pos < blk.length ? pos : -1;  // the last visible token
+    const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+    const float c = a.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    int vbuf = 1, guards = 0;
+    uint32_t vround = 0;
+    for (int j = 0; j < blk.n; ++j) {
+      const int first_key = blk.tiles.tile(j) * kTileKeys;
+      ok = wait_warp(&s_full[tile], j & 1u);
+      if (!ok) break;
+      ptx::tc_fence_after_sync();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32b_x32(t_s + q * 32, s[q]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) ptx::tmem_ld_wait_for(s[q]);
+      const bool masked = !whole(tile, first_key);
+      if (masked) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int k0 = first_key + q * 32;
+          const uint32_t see = (bit_range(lo - k0, last - k0) | bit_range(0, min(p.sinks - 1, last) - k0));
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (!(see & (1u << e))) s[q][e] = 0xff800000u;  // -inf
+          }
+        }
+      }
+      float top[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        top[q] = __uint_as_float(s[q][0]);
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top[q] = fmaxf(top[q], __uint_as_float(s[q][e]));
+      }
+      const float most = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+      const bool raise = (most - m) * c > kRaise;  // also from -inf to a number
+      if (__any_sync(0xffffffffu, raise)) {
+        const float factor = raise ? exp2_fast((m - most) * c) : 1.f;
+        if (raise) m = most;
+        l *= factor;
+        if (j > 0) {
+          // the products of the tile before must have arrived; the next ones wait for this tile's weights
+          ok = wait_warp(&o_done[tile], (j - 1) & 1u);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
+            ptx::tmem_ld_wait_for(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st_32x32b_x32(t_o + q * 32, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m * c;
+      float sum[4] = {};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
+          const float x = exp2_fast(__uint_as_float(src[0]) * c - base), y = exp2_fast(__uint_as_float(src[1]) * c - base);
+          sum[e & 3] += x + y;
+          w[e] = pack<BF16>(x, y);
+        }
+        tmem_st_32x32b_x32(t_s + half * 32, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      ptx::tc_fence_before_sync();
+      // A hidden token's weight is zero, and zero times infinity is not: tiles that are not seen whole have their values looked
+      // at (by both groups of warps, half of a tile each).  Tokens behind the length become zero; should any other be
+      // infinite or not a number, the rows of this CTA are computed one by one at the end.
+      if (masked || !whole(1 - tile, first_key)) {
+        ok = wait_warp(&kv_full[vbuf], vround & 1u);
+        if (!ok) break;
+        bool odd = false;
+#pragma unroll 1
+        for (int x = threadIdx.x; x < TILE / 16; x += kSoftmaxThreads) {
+          const uint32_t at = ring + vbuf * TILE + x * 16;
+          if (first_key + (x & (BLOCK / 16 - 1)) / 8 >= blk.length) {
+            ptx::st_shared_v4(at, make_uint4(0, 0, 0, 0));
+          } else {
+            const uint4 v = ptx::ld_shared_v4(at);
+            odd = odd || pair_not_finite<BF16>(v.x) || pair_not_finite<BF16>(v.y) || pair_not_finite<BF16>(v.z) ||
+                  pair_not_finite<BF16>(v.w);
+          }
+        }
+        if (odd) dirty = 1;
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&v_ok);
+        ++guards;
+      }
+      ptx::mbar_arrive(&p_full[tile]);
+      vbuf += 2;
+      if (vbuf >= NB) {
+        vbuf -= NB;
+        ++vround;
+      }
+    }
+    if (blk.n > 0 && ok) {
+      ok = wait_warp(&o_done[tile], (blk.n - 1) & 1u);
+      ptx::tc_fence_after_sync();
+    }
+    // everybody's findings are in: dirty, failed
+    ptx::named_barrier_sync(1, kSoftmaxThreads);
+    const bool by_rows = *const_cast<volatile int*>(&dirty) != 0, gave_up = *const_cast<volatile int*>(&failed) != 0;
+    uint16_t* dst = static_cast<uint16_t*>(p.out) +
+                    ((static_cast<long long>(blk.b) * p.sq + t) * p.heads + blk.kv_head * a.group + head) * D;
+    if (!by_rows || gave_up) {
+      const float inv = gave_up ? NAN : l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t o[32] = {};
+        if (blk.n > 0) {
+          ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
+          ptx::tmem_ld_wait_for(o);
+        }
+        if (real) {
+          // a row that sees nothing is zero, whatever its accumulator holds
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t w[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float f0 = __uint_as_float(o[e * 8 + x * 2]), f1 = __uint_as_float(o[e * 8 + x * 2 + 1]);
+              w[x] = inv == 0.f ? 0u : pack<BF16>(f0 * inv, f1 * inv);
+            }
+            ptx::st_v4(dst + q * 32 + e * 8, make_uint4(w[0], w[1], w[2], w[3]));
+          }
+        }
+      }
+    } else {
+      const int rows = a.group * a.tokens;
+      for (int r = warp; r < 2 * rows; r += kSoftmaxThreads / 32) {
+        const int tok = blk.t0 + r / a.group;
+        if (tok < p.sq) exact_row<D, BF16>(p, blk.b, tok, blk.kv_head * a.group + r % a.group, blk.length, c);
+      }
+    }
+    ptx::tc_fence_before_sync();
+  }
+  __syncthreads();
+  if (failed != 0) {
+    // a wait ran out: copies and products that are still under way get time to end before their memory is given back
+    const uint64_t until = ptx::globaltimer_ns() + 2000000ull;
+    while (ptx::globaltimer_ns() < until) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 8) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &found) == cudaSuccess &&
+                    found == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr) : nullptr;
+  }();
+  return fn;
+}
+// [d3, d2, d1, head_dim] of 16-bit values; strides in values.  A dimension that is broadcast (stride 0) becomes one entry.
+bool make_map(CUtensorMap* map, const void* base, DType dt, int head_dim, const int (&dims)[3], const long long (&strides)[3],
+              const int (&box)[2]) {
+  if (encode_fn() == nullptr) return false;
+  cuuint64_t size[4] = {static_cast<cuuint64_t>(head_dim), 1, 1, 1};
+  cuuint64_t bytes[3];
+  for (int d = 0; d < 3; ++d) {
+    size[d + 1] = strides[d] == 0 ? 1 : static_cast<cuuint64_t>(dims[d]);
+    bytes[d] = strides[d] == 0 ? 16 : static_cast<cuuint64_t>(strides[d]) * 2;
+  }
+  const cuuint32_t boxes[4] = {64, static_cast<cuuint32_t>(box[0]), static_cast<cuuint32_t>(box[1]), 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return encode_fn()(map, dt == DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                     const_cast<void*>(base), size, bytes, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Tensors that the copy engine cannot walk (tokens or query heads that are broadcast) and scales that are not positive (the
+// largest score is looked for before scaling) go row by row.
+bool fits_tiles(const PromptParams& p) {
+  const int group = p.heads / p.kv_heads;
+  return p.scale > 0 && (p.sk == 1 || (p.k_stride[1] != 0 && p.v_stride[1] != 0)) && (p.sq == 1 || p.q_stride[1] != 0) &&
+         (group == 1 || p.q_stride[2] != 0);
+}
+
+template <int D, bool BF16>
+cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
+  if (!fits_tiles(p)) {
+    const long long rows = static_cast<long long>(p.batch) * p.sq * p.heads;
+    const long long grid = std::min<long long>((rows + 7) / 8, 8ll * device_sm_count());
+    return launch_after(prompt_rows_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p);
+  }
+  PromptArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.p = p;
+  a.group = p.heads / p.kv_heads;
+  a.tokens = kTileRows / a.group;
+  a.blocks = (p.sq + 2 * a.tokens - 1) / (2 * a.tokens);
+  a.scale_log2 = p.scale * kLog2e;
+  a.q_batch = p.q_stride[0] != 0;
+  a.q_head = p.q_stride[2] != 0;
+  a.k_batch = p.k_stride[0] != 0;
+  a.k_head = p.k_stride[2] != 0;
+  a.v_batch = p.v_stride[0] != 0;
+  a.v_head = p.v_stride[2] != 0;
+  if (!make_map(&a.q, p.q, dt, D, {p.heads, p.sq, p.batch}, {p.q_stride[2], p.q_stride[1], p.q_stride[0]},
+                {a.group, a.tokens}) ||
+      !make_map(&a.k, p.k, dt, D, {p.sk, p.kv_heads, p.batch}, {p.k_stride[1], p.k_stride[2], p.k_stride[0]}, {kTileKeys, 1}) ||
+      !make_map(&a.v, p.v, dt, D, {p.sk, p.kv_heads, p.batch}, {p.v_stride[1], p.v_stride[2], p.v_stride[0]}, {kTileKeys, 1})) {
+    return cudaErrorInvalidValue;
+  }
+  const long long grid = static_cast<long long>(a.blocks) * p.batch * p.kv_heads;
+  if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(prompt_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       prompt_smem_bytes<D>());
+  if (e != cudaSuccess) return e;
+  return launch_after(prompt_attention_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), kPromptThreads,
+                      prompt_smem_bytes<D>(), stream, a);
 }
 
 }  // namespace
 
 cudaError_t launch_prompt_attention(const PromptParams& p, DType dt, cudaStream_t stream) {
   if (p.batch == 0 || p.sq == 0) return cudaSuccess;
-  if (p.head_dim == 128) return dt == DT_BF16 ? launch_typed<128, true>(p, stream) : launch_typed<128, false>(p, stream);
-  if (p.head_dim == 64) return dt == DT_BF16 ? launch_typed<64, true>(p, stream) : launch_typed<64, false>(p, stream);
+  if (p.head_dim == 128) return dt == DT_BF16 ? launch_typed<128, true>(p, dt, stream) : launch_typed<128, false>(p, dt, stream);
+  if (p.head_dim == 64) return dt == DT_BF16 ? launch_typed<64, true>(p, dt, stream) : launch_typed<64, false>(p, dt, stream);
   return cudaErrorInvalidValue;
 }
 
