@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const __grid_constant_
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr uint64_t kDeadlineNs = 4000000000ull;  // of a wait; nothing here takes a thousandth of it
+constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
+constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
 
 template <int D>
@@ -153,6 +155,18 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
       : "memory");
 }
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(e));
+  return e != 0;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bits lo .. hi (inclusive) of a 32-bit word; none if hi < lo.
@@ -167,6 +181,14 @@ __device__ __forceinline__ bool pair_not_finite(uint32_t u) {
   return (u & e) == e || (u & (e << 16)) == (e << 16);
 }
 
+// Scores whose bit is not set become -inf.
+__device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t see) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) {
+    if (!(see & (1u << e))) s[e] = 0xff800000u;
+  }
+}
+
 // What a CTA works on.
 struct PromptBlock {
   int b, kv_head, t0, length;  // first token of the first tile
@@ -179,7 +201,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   constexpr int NB = ring_buffers<D>(), TILE = key_tile_bytes<D>(), BLOCK = kTileKeys * 128;
   const PromptParams& p = a.p;
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ __align__(8) uint64_t q_full[2], kv_full[NB], kv_empty[NB], s_full[2], p_full[2], o_done[2], v_ok;
+  __shared__ __align__(8) uint64_t q_full[2], kv_full[NB], kv_empty[NB], s_full[2], p_full[2][2], o_done[2], v_ok;
   __shared__ uint32_t tmem_slot;
   __shared__ int failed, dirty;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -190,7 +212,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&q_full[i], 1);
       ptx::mbar_init(&s_full[i], 1);
-      ptx::mbar_init(&p_full[i], kTileRows);
+      ptx::mbar_init(&p_full[i][0], kTileRows);
+      ptx::mbar_init(&p_full[i][1], kTileRows);
       ptx::mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < NB; ++i) {
@@ -288,27 +311,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     __syncwarp();
   } else if (warp == 9) {
     hand_over();
-    if (lane == 0 && blk.n > 0) {
+    if (blk.n > 0) {
+      // The whole warp walks the tiles; one lane issues.
       constexpr int FMT = BF16 ? 1 : 0;
       constexpr uint32_t idesc_s = ptx::make_idesc_f16(FMT, kTileRows, kTileKeys);
       constexpr uint32_t idesc_o = ptx::make_idesc_f16(FMT, kTileRows, D) | (1u << 16);  // B along its rows
-      auto scores = [&](int i, uint32_t keys) {
+      const uint64_t desc_q = ptx::make_smem_desc_k_sw128(smem), desc_k = ptx::make_smem_desc_k_sw128(ring);
+      const uint64_t desc_v = make_smem_desc_mn_sw128(ring, BLOCK);
+      auto scores = [&](int i, int buffer) {
+        const uint64_t q = desc_q + i * ((D / 64) * (kTileRows * 128) / 16), k = desc_k + buffer * (TILE / 16);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * BLOCK + (k & 3) * 32;
-          ptx::umma_f16_ss(tmem + i * kTileKeys,
-                           ptx::make_smem_desc_k_sw128(smem + i * (D / 64) * (kTileRows * 128) + off),
-                           ptx::make_smem_desc_k_sw128(keys + off), idesc_s, k > 0);
+        for (int x = 0; x < D / 16; ++x) {
+          constexpr int kStep = 32 / 16;
+          const int off = (x >> 2) * (BLOCK / 16) + (x & 3) * kStep;
+          ptx::umma_f16_ss(tmem + i * kTileKeys, q + off, k + off, idesc_s, x > 0);
         }
         ptx::umma_commit(&s_full[i]);
       };
-      auto outputs = [&](int i, uint32_t values, bool first) {
+      auto outputs = [&](int i, int half, int buffer, bool first) {
+        const uint64_t v = desc_v + buffer * (TILE / 16);
 #pragma unroll
-        for (int k = 0; k < kTileKeys / 16; ++k) {
-          umma_f16_ts(tmem + 2 * kTileKeys + i * 128, tmem + i * kTileKeys + k * 8,
-                      make_smem_desc_mn_sw128(values + k * 16 * 128, BLOCK), idesc_o, !first || k > 0);
+        for (int y = 0; y < kTileKeys / 32; ++y) {
+          const int x = half * (kTileKeys / 32) + y;
+          umma_f16_ts(tmem + 2 * kTileKeys + i * 128, tmem + i * kTileKeys + x * 8, v + x * (16 * 128 / 16), idesc_o,
+                      !first || x > 0);
         }
-        ptx::umma_commit(&o_done[i]);
       };
       int buf = 0;
       uint32_t round = 0, guards = 0;
@@ -318,45 +345,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           ++round;
         }
       };
-      bool ok = true;
+      bool ok = wait_warp(&kv_full[0], 0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        ok = ok && wait(&q_full[i], 0);
-        if (i == 0) ok = ok && wait(&kv_full[0], 0);
-        if (ok) scores(i, ring);
+        ok = ok && wait_warp(&q_full[i], 0);
+        if (ok && elect_one()) {
+          scores(i, 0);
+          if (i == 1) ptx::umma_commit(&kv_empty[0]);
+        }
+        __syncwarp();
       }
-      if (ok) ptx::umma_commit(&kv_empty[0]);
       next();
       for (int j = 0; ok && j < blk.n; ++j) {
         const int first_key = blk.tiles.tile(j) * kTileKeys;
         const int vbuf = buf;
-        ok = wait(&kv_full[vbuf], round & 1u);
+        ok = wait_warp(&kv_full[vbuf], round & 1u);
         next();
         const int kbuf = buf;
         const bool more = j + 1 < blk.n;
         if (ok && more) {
-          ok = wait(&kv_full[kbuf], round & 1u);
+          ok = wait_warp(&kv_full[kbuf], round & 1u);
           next();
         }
         if (ok && !(whole(0, first_key) && whole(1, first_key))) {
-          ok = wait(&v_ok, guards & 1u);
+          ok = wait_warp(&v_ok, guards & 1u);
           ++guards;
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          ok = ok && wait(&p_full[i], j & 1u);
+          // the first half of the products starts while the second half of the weights is computed
+          ok = ok && wait_warp(&p_full[i][0], j & 1u);
           if (!ok) break;
           ptx::tc_fence_after_sync();
-          outputs(i, ring + vbuf * TILE, j == 0);
-          if (i == 1) ptx::umma_commit(&kv_empty[vbuf]);
-          if (more) {
-            scores(i, ring + kbuf * TILE);
-            if (i == 1) ptx::umma_commit(&kv_empty[kbuf]);
+          if (elect_one()) outputs(i, 0, vbuf, j == 0);
+          __syncwarp();
+          ok = wait_warp(&p_full[i][1], j & 1u);
+          if (!ok) break;
+          ptx::tc_fence_after_sync();
+          if (elect_one()) {
+            outputs(i, 1, vbuf, j == 0);
+            ptx::umma_commit(&o_done[i]);
+            if (i == 1) ptx::umma_commit(&kv_empty[vbuf]);
+            if (more) {
+              scores(i, kbuf);
+              if (i == 1) ptx::umma_commit(&kv_empty[kbuf]);
+            }
           }
+          __syncwarp();
         }
       }
     }
-    __syncwarp();
   } else if (warp >= 10) {
     hand_over();
   } else {
@@ -372,7 +410,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     const int last = real && pos < blk.length ? pos : -1;  // the last visible token
     const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
     const float c = a.scale_log2;
-    float m = -INFINITY, l = 0.f;
+    float m = kLowest, l = 0.f;
     bool ok = true;
     int vbuf = 1, guards = 0;
     uint32_t vround = 0;
@@ -391,22 +429,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int k0 = first_key + q * 32;
-          const uint32_t see = (bit_range(lo - k0, last - k0) | bit_range(0, min(p.sinks - 1, last) - k0));
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            if (!(see & (1u << e))) s[q][e] = 0xff800000u;  // -inf
-          }
+          hide(s[q], bit_range(lo - k0, last - k0) | bit_range(0, min(p.sinks - 1, last) - k0));
         }
       }
+      // (NaN counts as the largest: it makes all of its row NaN)
       float top[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        top[q] = __uint_as_float(s[q][0]);
+      for (int q = 0; q < 4; ++q) top[q] = __uint_as_float(s[q][0]);
 #pragma unroll
-        for (int e = 1; e < 32; ++e) top[q] = fmaxf(top[q], __uint_as_float(s[q][e]));
+      for (int e = 1; e < 31; e += 2) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) top[q] = max3_nan(top[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
       }
-      const float most = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
-      const bool raise = (most - m) * c > kRaise;  // also from -inf to a number
+      top[0] = max3_nan(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+      top[1] = max3_nan(top[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
+      const float most = max3_nan(max3_nan(top[0], top[1], m), top[2], top[3]);
+      const bool raise = real && !((most - m) * c <= kRaise);  // also for NaN; rows that no token fills hold anything
       if (__any_sync(0xffffffffu, raise)) {
         const float factor = raise ? exp2_fast((m - most) * c) : 1.f;
         if (raise) m = most;
@@ -428,23 +466,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           tmem_st_wait();
         }
       }
-      const float base = m == -INFINITY ? 0.f : m * c;
-      float sum[4] = {};
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
-          const float x = exp2_fast(__uint_as_float(src[0]) * c - base), y = exp2_fast(__uint_as_float(src[1]) * c - base);
-          sum[e & 3] += x + y;
-          w[e] = pack<BF16>(x, y);
-        }
-        tmem_st_32x32b_x32(t_s + half * 32, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      ptx::tc_fence_before_sync();
       // A hidden token's weight is zero, and zero times infinity is not: tiles that are not seen whole have their values looked
       // at (by both groups of warps, half of a tile each).  Tokens behind the length become zero; should any other be
       // infinite or not a number, the rows of this CTA are computed one by one at the end.
@@ -468,7 +489,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         ptx::mbar_arrive(&v_ok);
         ++guards;
       }
-      ptx::mbar_arrive(&p_full[tile]);
+      float base = m == kLowest ? 0.f : m * c;
+      base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
+      const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
+      Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
+          const Pair x = fma2(make_pair(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, base2);
+          float2 y;
+          if (e % kPolyEvery == kPolyEvery - 1) {
+            y = exp2_poly(x);
+          } else {
+            y = split(x);
+            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+          }
+          sum[e & 1] = add2(sum[e & 1], make_pair(y.x, y.y));
+          w[e] = pack<BF16>(y.x, y.y);
+        }
+        tmem_st_32x32b_x32(t_s + half * 32, w);
+        tmem_st_wait();
+        ptx::tc_fence_before_sync();
+        ptx::mbar_arrive(&p_full[tile][half]);
+      }
+      const float2 total = split(add2(sum[0], sum[1]));
+      l += total.x + total.y;
       vbuf += 2;
       if (vbuf >= NB) {
         vbuf -= NB;
