@@ -189,7 +189,7 @@ static void paged_attention_op(at::Tensor q, at::Tensor cache, at::Tensor page_t
   check_apart(out, page_table, "out", "page_table");
   check_apart(out, lengths, "out", "lengths");
   const int64_t width = page_table.size(1);
-  TORCH_CHECK(seqs * heads * (width * p.pages.page_size / 64 + 1) <= std::numeric_limits<int>::max(),
+  TORCH_CHECK(seqs * heads * (width * p.pages.page_size / 64 + 3) <= std::numeric_limits<int>::max(),
               "too many tokens in one call");
   p.q = q.data_ptr();
   p.cache = cache.data_ptr();
@@ -329,14 +329,15 @@ static std::vector<int64_t> page_place_op(std::vector<int64_t> row, int64_t pos,
   const int page = l.find(r.data(), static_cast<int>(r.size()), static_cast<int>(pos), place);
   return {page, place, page < 0 ? -1 : l.key_offset(page, static_cast<int>(head), place)};
 }
-// The tiles of `tile` tokens that the positions [p0, p1] of a sequence look at, by the function the kernels use.
+// First tokens of the tiles of `tile` tokens that the positions [p0, p1] of a sequence look at, by the function the kernels use.
 static std::vector<int64_t> seen_tiles_op(int64_t p0, int64_t p1, int64_t length, int64_t window, int64_t sinks, int64_t tile) {
-  TORCH_CHECK(p0 <= p1 && p1 < std::numeric_limits<int>::max() && length >= 0 && tile > 0, "seen_tiles: bad arguments");
+  TORCH_CHECK(p0 >= -1 && p0 <= p1 && p1 < std::numeric_limits<int>::max() && length >= 0 &&
+                  length <= std::numeric_limits<int>::max() - 1024 && tile > 0 && tile <= 1024, "seen_tiles: bad arguments");
   check_window(window, sinks);
   const SeenTiles t = seen_tiles(static_cast<int>(p0), static_cast<int>(p1), static_cast<int>(length),
                                  static_cast<int>(window), static_cast<int>(sinks), static_cast<int>(tile));
   std::vector<int64_t> out;
-  for (int i = 0; i < t.count(); ++i) out.push_back(t.tile(i));
+  for (int i = 0; i < t.count(); ++i) out.push_back(t.start(i));
   return out;
 }
 

@@ -59,23 +59,26 @@ struct PageLayout {
   }
 };
 
-// The tokens that one position sees, in tiles of `tile` tokens: [0, n_sink) and [first, end).
+// Tiles of `tile` tokens: the first n_sink of the sequence, then n from token `first` on.
 struct SeenTiles {
-  int n_sink, first, end;
-  __host__ __device__ int count() const { return n_sink + end - first; }
-  __host__ __device__ int tile(int i) const { return i < n_sink ? i : first + (i - n_sink); }
+  int n_sink, first, n, tile;
+  __host__ __device__ int count() const { return n_sink + n; }
+  __host__ __device__ int start(int i) const { return i < n_sink ? i * tile : first + (i - n_sink) * tile; }
 };
-// Tiles of the tokens that some position of [p0, p1] sees in a sequence of `length` tokens, p0 <= p1 < length.
+// The tiles that hold the tokens which some position of [p0, p1] sees in a sequence of `length` tokens, p0 <= p1.  A window's
+// tiles begin with the first token it shows, wherever that is, and not at a multiple of the tile.
 __host__ __device__ inline SeenTiles seen_tiles(int p0, int p1, int length, int window, int sinks, int tile) {
   SeenTiles t;
-  const int last = p1 < length ? p1 : length - 1;  // the last visible token
-  t.end = last < 0 ? 0 : last / tile + 1;
+  const int end = p1 < length ? p1 + 1 : length;  // behind the last visible token
   // (p0 - window may be far below zero, never below the smallest int)
   const int lo = window > 0 && p0 >= window ? p0 - window + 1 : 0;
-  t.first = lo / tile < t.end ? lo / tile : t.end;
-  const int sink = sinks < lo ? sinks : lo;  // visible tokens in front of the window
-  t.n_sink = window > 0 && sink > 0 ? (sink - 1) / tile + 1 : 0;
-  if (t.n_sink > t.first) t.n_sink = t.first;
+  int sink = sinks < lo ? sinks : lo;  // visible tokens in front of the window
+  if (sink > end) sink = end;
+  t.tile = tile;
+  t.n_sink = sink > 0 ? (sink - 1) / tile + 1 : 0;
+  const int behind = t.n_sink * tile;  // (below the largest int: a tile more than a length of at most 2^31 - 1024)
+  t.first = lo > behind ? lo : behind;
+  t.n = end > t.first ? (end - t.first - 1) / tile + 1 : 0;
   return t;
 }
 __host__ __device__ inline bool is_visible(int i, int j, int length, int window, int sinks) {

@@ -87,7 +87,7 @@ __device__ __forceinline__ Sequence sequence(const PagedParams& p, int s) {
 struct Cursor {
   int s, head, i, left;  // sequence, virtual head, tile of the sequence, tiles to go in this CTA
   Sequence q;
-  __device__ __forceinline__ int tile() const { return q.t.tile(i); }
+  __device__ __forceinline__ int first_token() const { return q.t.start(i); }
   __device__ __forceinline__ void advance(const PagedParams& p, int heads) {
     --left;
     if (++i < q.count) return;
@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     page = -1;
     bad = false;
     if (ic.left > 0) {
-      const int pos = ic.tile() * kTile + warp * kStrip + (lane & (kStrip - 1));
+      const int pos = ic.first_token() + warp * kStrip + (lane & (kStrip - 1));
       if (is_visible(ic.q.length - 1, pos, ic.q.length, p.window, p.sinks)) {
         page = p.pages.find(p.table + ic.s * p.table_stride, p.width, pos, place);
         bad = page < 0;
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         mma_16x8x16<BF16>(c[1], qf[ks], b[2], b[3]);
       }
     }
-    const int pos0 = cc.tile() * kTile + warp * kStrip;
+    const int pos0 = cc.first_token() + warp * kStrip;
     float top[2] = {m[0], m[1]};
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {

@@ -7,9 +7,16 @@
 // compute the weights of the other.
 //
 //   warps 0-3, 4-7   softmax of the two tiles: warp w reads the TMEM lanes 32 (w % 4) .. + 31, a thread is a row
-//   warp 8           TMA: Q once, then K and V tile by tile into a ring of buffers
+//   warp 8           TMA: Q, then K and V tile by tile into a ring of buffers
 //   warp 9           tcgen05.mma: S_i = Q_i K_j^T from shared memory, O_i += P_i V_j with P_i in TMEM
-//   warps 10, 11     none (registers are handed over by four warps at a time)
+//   warps 10, 11     look at the values of tiles that are not seen whole (below)
+//
+// A CTA that has loaded the last keys of its pair of tiles asks the hardware for a CTA that has not been launched yet and
+// takes its place (clusterlaunchcontrol): its loads and first scores run under the last weights and the stores of the
+// pair before.  Pairs with the most keys are launched first.
+//
+// A hidden token's weight is zero, and zero times infinity is not: in tiles that some row does not see whole, values behind
+// the length become zero, and should any other not be finite, the rows of the pair are computed one by one at the end.
 //
 // TMEM (512 columns of 32 bits): S_0, S_1 (128 each; P_i, 16-bit pairs, over the first 64 of S_i), O_0, O_1 (head_dim each).
 //
@@ -95,16 +102,17 @@ constexpr float kRaise = 8.f;                    // powers of two that a row's l
 
 template <int D>
 constexpr int ring_buffers() {
-  return D == 128 ? 5 : 8;
+  return D == 128 ? 4 : 8;
 }
 template <int D>
 constexpr int key_tile_bytes() {
   return kTileKeys * D * 2;
 }
-// shared memory behind the first 1024-byte boundary: two Q tiles, then the ring
+constexpr int kStageBytes = 32 * 128;  // 64 columns of a warp's results, on their way out
+// shared memory behind the first 1024-byte boundary: two Q tiles, the ring, a stage for each softmax warp
 template <int D>
 constexpr int prompt_smem_bytes() {
-  return 2 * kTileRows * D * 2 + ring_buffers<D>() * key_tile_bytes<D>() + 1024;
+  return 2 * kTileRows * D * 2 + ring_buffers<D>() * key_tile_bytes<D>() + 8 * kStageBytes + 1024;
 }
 
 struct PromptArgs {
@@ -175,10 +183,17 @@ __device__ __forceinline__ uint32_t bit_range(int lo, int hi) {
   hi = min(hi, 31);
   return hi < lo ? 0u : (0xffffffffu >> (31 - hi)) & (0xffffffffu << lo);
 }
+// Largest magnitude of two 16-bit values, as integers: infinities and NaN are the largest of all.
+__device__ __forceinline__ uint32_t magnitudes(uint32_t m, const uint4& v) {
+  m = __vmaxu2(m, v.x & 0x7fff7fffu);
+  m = __vmaxu2(m, v.y & 0x7fff7fffu);
+  m = __vmaxu2(m, v.z & 0x7fff7fffu);
+  return __vmaxu2(m, v.w & 0x7fff7fffu);
+}
 template <bool BF16>
-__device__ __forceinline__ bool pair_not_finite(uint32_t u) {
-  constexpr uint32_t e = BF16 ? 0x7f80u : 0x7c00u;
-  return (u & e) == e || (u & (e << 16)) == (e << 16);
+__device__ __forceinline__ bool all_finite(uint32_t m) {
+  constexpr uint32_t inf = BF16 ? 0x7f80u : 0x7c00u;
+  return (m & 0xffffu) < inf && (m >> 16) < inf;
 }
 
 // Scores whose bit is not set become -inf.
@@ -189,24 +204,94 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t see) {
   }
 }
 
-// What a CTA works on.
-struct PromptBlock {
-  int b, kv_head, t0, length;  // first token of the first tile
+// What a CTA works on: a pair of tiles.
+struct PromptPair {
+  int b, kv_head, t0, length;  // t0: first token of the first tile
   SeenTiles tiles;
   int n;  // tiles of keys; 0: no row sees anything
 };
+__device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index) {
+  const PromptParams& p = a.p;
+  PromptPair r;
+  // late tokens first: they see the most keys
+  const int per = p.batch * p.kv_heads;
+  const int qb = index / per, rest = index - qb * per;
+  r.b = rest / p.kv_heads;
+  r.kv_head = rest - r.b * p.kv_heads;
+  r.t0 = (a.blocks - 1 - qb) * 2 * a.tokens;
+  r.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + r.b), 0), p.sk);
+  const int p0 = p.sk - p.sq + r.t0, p1 = p.sk - p.sq + min(r.t0 + 2 * a.tokens, p.sq) - 1;
+  r.tiles = seen_tiles(p0, p1, r.length, p.window, p.sinks, kTileKeys);
+  r.n = p0 < r.length ? r.tiles.count() : 0;
+  return r;
+}
+// Whether every row of tile i (0, 1) sees all of a tile of keys.
+__device__ __forceinline__ bool sees_whole(const PromptArgs& a, const PromptPair& r, int i, int first_key) {
+  const PromptParams& p = a.p;
+  const int lo = p.sk - p.sq + r.t0 + i * a.tokens, hi = min(lo + a.tokens, p.sk) - 1, last_key = first_key + kTileKeys - 1;
+  return last_key <= lo && last_key < r.length && hi < r.length &&
+         (p.window == 0 || hi - first_key < p.window || last_key < p.sinks);
+}
+__device__ __forceinline__ bool seen_by_all(const PromptArgs& a, const PromptPair& r, int first_key) {
+  return sees_whole(a, r, 0, first_key) && sees_whole(a, r, 1, first_key);
+}
+
+// A place in a ring of N buffers, and how often the ring has been gone round.
+template <int N>
+struct Ring {
+  int at = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next(int n = 1) {
+    at += n;
+    if (at >= N) {
+      at -= N;
+      ++round;
+    }
+  }
+};
+
+// Asks for a CTA that has not been launched; the answer (16 bytes) arrives on `bar`.
+__device__ __forceinline__ void claim_cta(void* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(ptx::smem_u32(answer)), "r"(ptx::smem_u32(bar))
+               : "memory");
+}
+// Index of the claimed CTA, -1 if there was none left.
+__device__ __forceinline__ int claimed_cta(const void* answer) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      ".reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t"
+      "}"
+      : "=r"(ok), "=r"(x)
+      : "r"(ptx::smem_u32(answer))
+      : "memory");
+  return ok ? static_cast<int>(x) : -1;
+}
+
+constexpr int kChecks = 8;    // tiles of values that may have been looked at and not used: more than the ring holds
+constexpr int kReaders = 12;  // of an answer: TMA, MMA, the two warps that look at values, eight softmax warps
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(const __grid_constant__ PromptArgs a) {
   constexpr int NB = ring_buffers<D>(), TILE = key_tile_bytes<D>(), BLOCK = kTileKeys * 128;
   const PromptParams& p = a.p;
   extern __shared__ __align__(128) uint8_t raw[];
-  __shared__ __align__(8) uint64_t q_full[2], kv_full[NB], kv_empty[NB], s_full[2], p_full[2][2], o_done[2], v_ok;
+  __shared__ __align__(16) uint4 answers[2];
+  __shared__ __align__(8) uint64_t q_full[2], q_empty, kv_full[NB], kv_empty[NB], s_full[2], p_full[2][2], o_done[2], v_ok[kChecks],
+      checked[2], next_full[2], next_empty[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int failed, dirty;
+  __shared__ int odd_pair[2];                            // the last pair (counted from 1) whose values are not all finite
+  __shared__ int failed, unfinished, taken, pending, pairs[4];  // after a wait that ran out, see the end
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (ptx::smem_u32(raw) + 1023u) & ~1023u;
-  const uint32_t ring = smem + 2 * kTileRows * D * 2;
+  const uint32_t ring = smem + 2 * kTileRows * D * 2, stage = ring + NB * TILE;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -215,16 +300,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       ptx::mbar_init(&p_full[i][0], kTileRows);
       ptx::mbar_init(&p_full[i][1], kTileRows);
       ptx::mbar_init(&o_done[i], 1);
+      ptx::mbar_init(&checked[i], 2);
+      ptx::mbar_init(&next_full[i], 1);
+      ptx::mbar_init(&next_empty[i], kReaders);
+      odd_pair[i] = 0;
     }
     for (int i = 0; i < NB; ++i) {
       ptx::mbar_init(&kv_full[i], 1);
       ptx::mbar_init(&kv_empty[i], 1);
     }
-    ptx::mbar_init(&v_ok, kSoftmaxThreads);
+    for (int i = 0; i < kChecks; ++i) ptx::mbar_init(&v_ok[i], 2);
+    ptx::mbar_init(&q_empty, 1);
     ptx::mbar_fence_init();
     ptx::fence_proxy_async_smem();
     failed = 0;
-    dirty = 0;
+    unfinished = INT32_MAX;
+    taken = 0;
+    pending = -1;
   }
   if (warp == 8) {
     if (lane == 0) {
@@ -242,144 +334,155 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const uint32_t tmem = tmem_slot;
   ptx::wait_for_previous_kernel();
 
-  PromptBlock blk;
-  {
-    // late tokens first: they see the most keys
-    const int per = p.batch * p.kv_heads;
-    const int qb = blockIdx.x / per, rest = blockIdx.x - qb * per;
-    blk.b = rest / p.kv_heads;
-    blk.kv_head = rest - blk.b * p.kv_heads;
-    blk.t0 = (a.blocks - 1 - qb) * 2 * a.tokens;
-    blk.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + blk.b), 0), p.sk);
-    const int p0 = p.sk - p.sq + blk.t0, p1 = p.sk - p.sq + min(blk.t0 + 2 * a.tokens, p.sq) - 1;
-    blk.tiles = seen_tiles(p0, p1, blk.length, p.window, p.sinks, kTileKeys);
-    blk.n = p0 < blk.length ? blk.tiles.count() : 0;
-  }
-  // Whether every row of tile i (0, 1) sees all of a tile of keys; if not, scores are masked and the values are looked at.
-  auto whole = [&](int i, int first_key) {
-    const int lo = p.sk - p.sq + blk.t0 + i * a.tokens, hi = min(lo + a.tokens, p.sk) - 1, last_key = first_key + kTileKeys - 1;
-    return last_key <= lo && last_key < blk.length && hi < blk.length &&
-           (p.window == 0 || hi - first_key < p.window || last_key < p.sinks);
-  };
   const uint64_t deadline = ptx::globaltimer_ns() + kDeadlineNs;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (ptx::mbar_wait(bar, parity, deadline)) return true;
-    failed = 1;
+    *const_cast<volatile int*>(&failed) = 1;
     return false;
   };
   // the lanes of a warp go on, or give up, together
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+  // The pair after the it-th; -1: none, or given up.
+  auto next_pair = [&](int it) {
+    if (!wait_warp(&next_full[it & 1], (it >> 1) & 1u)) return -1;
+    const int index = claimed_cta(&answers[it & 1]);
+    __syncwarp();
+    if (lane == 0) {
+      ptx::fence_proxy_async_smem();
+      ptx::mbar_arrive(&next_empty[it & 1]);
+    }
+    return index;
+  };
 
   // 384 threads x 168 registers at launch = 128 x 56 + 256 x 224
   auto hand_over = [] { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); };
   if (warp == 8) {
     hand_over();
-    if (lane == 0 && blk.n > 0) {
+    if (lane == 0) {
       const int rows = a.group * a.tokens;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ptx::mbar_arrive_expect_tx(&q_full[i], rows * D * 2);
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-          tma_load_4d(smem + (i * (D / 64) + c) * (kTileRows * 128), &a.q, &q_full[i], c * 64,
-                      blk.kv_head * a.group * a.q_head, blk.t0 + i * a.tokens, blk.b * a.q_batch);
-        }
-      }
-      int buf = 0;
-      uint32_t round = 0;
-      for (int j = 0; j < blk.n; ++j) {
-        const int key = blk.tiles.tile(j) * kTileKeys;
-        bool ok = true;
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (round > 0) ok = ok && wait(&kv_empty[buf], (round - 1) & 1u);
-          if (!ok) break;
-          ptx::mbar_arrive_expect_tx(&kv_full[buf], TILE);
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c) {
-            tma_load_4d(ring + buf * TILE + c * BLOCK, kv == 0 ? &a.k : &a.v, &kv_full[buf], c * 64, key,
-                        blk.kv_head * (kv == 0 ? a.k_head : a.v_head), blk.b * (kv == 0 ? a.k_batch : a.v_batch));
-          }
-          if (++buf == NB) {
-            buf = 0;
-            ++round;
-          }
-        }
+      Ring<NB> buf;
+      bool ok = true;
+      uint32_t loaded = 0;  // pairs with keys
+      int index = blockIdx.x;
+      for (int it = 0;; ++it) {
+        const int slot = it & 1;
+        pairs[it & 3] = index;
+        *const_cast<volatile int*>(&taken) = it + 1;
+        if (it >= 2) ok = wait(&next_empty[slot], ((it >> 1) - 1) & 1u);
         if (!ok) break;
+        *const_cast<volatile int*>(&pending) = it;
+        ptx::mbar_arrive_expect_tx(&next_full[slot], 16);
+        claim_cta(&answers[slot], &next_full[slot]);
+        const PromptPair r = prompt_pair(a, index);
+        if (r.n > 0) {
+          if (loaded > 0) ok = wait(&q_empty, (loaded - 1) & 1u);
+          if (!ok) break;
+          ++loaded;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ptx::mbar_arrive_expect_tx(&q_full[i], rows * D * 2);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              tma_load_4d(smem + (i * (D / 64) + c) * (kTileRows * 128), &a.q, &q_full[i], c * 64,
+                          r.kv_head * a.group * a.q_head, r.t0 + i * a.tokens, r.b * a.q_batch);
+            }
+          }
+        }
+        for (int j = 0; ok && j < r.n; ++j) {
+          const int key = r.tiles.start(j);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            if (buf.round > 0) ok = ok && wait(&kv_empty[buf.at], (buf.round - 1) & 1u);
+            if (!ok) break;
+            ptx::mbar_arrive_expect_tx(&kv_full[buf.at], TILE);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+              tma_load_4d(ring + buf.at * TILE + c * BLOCK, kv == 0 ? &a.k : &a.v, &kv_full[buf.at], c * 64, key,
+                          r.kv_head * (kv == 0 ? a.k_head : a.v_head), r.b * (kv == 0 ? a.k_batch : a.v_batch));
+            }
+            buf.next();
+          }
+        }
+        ok = ok && wait(&next_full[slot], (it >> 1) & 1u);
+        if (!ok) break;
+        index = claimed_cta(&answers[slot]);
+        *const_cast<volatile int*>(&pending) = -1;
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(&next_empty[slot]);
+        if (index < 0) break;
       }
+      ptx::allow_next_kernel();
     }
     __syncwarp();
   } else if (warp == 9) {
     hand_over();
-    if (blk.n > 0) {
-      // The whole warp walks the tiles; one lane issues.
-      constexpr int FMT = BF16 ? 1 : 0;
-      constexpr uint32_t idesc_s = ptx::make_idesc_f16(FMT, kTileRows, kTileKeys);
-      constexpr uint32_t idesc_o = ptx::make_idesc_f16(FMT, kTileRows, D) | (1u << 16);  // B along its rows
-      const uint64_t desc_q = ptx::make_smem_desc_k_sw128(smem), desc_k = ptx::make_smem_desc_k_sw128(ring);
-      const uint64_t desc_v = make_smem_desc_mn_sw128(ring, BLOCK);
-      auto scores = [&](int i, int buffer) {
-        const uint64_t q = desc_q + i * ((D / 64) * (kTileRows * 128) / 16), k = desc_k + buffer * (TILE / 16);
+    // The whole warp walks the tiles; one lane issues.
+    constexpr int FMT = BF16 ? 1 : 0;
+    constexpr uint32_t idesc_s = ptx::make_idesc_f16(FMT, kTileRows, kTileKeys);
+    constexpr uint32_t idesc_o = ptx::make_idesc_f16(FMT, kTileRows, D) | (1u << 16);  // B along its rows
+    const uint64_t desc_q = ptx::make_smem_desc_k_sw128(smem), desc_k = ptx::make_smem_desc_k_sw128(ring);
+    const uint64_t desc_v = make_smem_desc_mn_sw128(ring, BLOCK);
+    auto scores = [&](int i, int buffer) {
+      const uint64_t q = desc_q + i * ((D / 64) * (kTileRows * 128) / 16), k = desc_k + buffer * (TILE / 16);
 #pragma unroll
-        for (int x = 0; x < D / 16; ++x) {
-          constexpr int kStep = 32 / 16;
-          const int off = (x >> 2) * (BLOCK / 16) + (x & 3) * kStep;
-          ptx::umma_f16_ss(tmem + i * kTileKeys, q + off, k + off, idesc_s, x > 0);
-        }
-        ptx::umma_commit(&s_full[i]);
-      };
-      auto outputs = [&](int i, int half, int buffer, bool first) {
-        const uint64_t v = desc_v + buffer * (TILE / 16);
-#pragma unroll
-        for (int y = 0; y < kTileKeys / 32; ++y) {
-          const int x = half * (kTileKeys / 32) + y;
-          umma_f16_ts(tmem + 2 * kTileKeys + i * 128, tmem + i * kTileKeys + x * 8, v + x * (16 * 128 / 16), idesc_o,
-                      !first || x > 0);
-        }
-      };
-      int buf = 0;
-      uint32_t round = 0, guards = 0;
-      auto next = [&] {
-        if (++buf == NB) {
-          buf = 0;
-          ++round;
-        }
-      };
-      bool ok = wait_warp(&kv_full[0], 0);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ok = ok && wait_warp(&q_full[i], 0);
-        if (ok && elect_one()) {
-          scores(i, 0);
-          if (i == 1) ptx::umma_commit(&kv_empty[0]);
-        }
-        __syncwarp();
+      for (int x = 0; x < D / 16; ++x) {
+        const int off = (x >> 2) * (BLOCK / 16) + (x & 3) * (32 / 16);
+        ptx::umma_f16_ss(tmem + i * kTileKeys, q + off, k + off, idesc_s, x > 0);
       }
-      next();
-      for (int j = 0; ok && j < blk.n; ++j) {
-        const int first_key = blk.tiles.tile(j) * kTileKeys;
-        const int vbuf = buf;
-        ok = wait_warp(&kv_full[vbuf], round & 1u);
-        next();
-        const int kbuf = buf;
-        const bool more = j + 1 < blk.n;
-        if (ok && more) {
-          ok = wait_warp(&kv_full[kbuf], round & 1u);
-          next();
+      ptx::umma_commit(&s_full[i]);
+    };
+    auto outputs = [&](int i, int half, int buffer, bool first) {
+      const uint64_t v = desc_v + buffer * (TILE / 16);
+#pragma unroll
+      for (int y = 0; y < kTileKeys / 32; ++y) {
+        const int x = half * (kTileKeys / 32) + y;
+        umma_f16_ts(tmem + 2 * kTileKeys + i * 128, tmem + i * kTileKeys + x * 8, v + x * (16 * 128 / 16), idesc_o,
+                    !first || x > 0);
+      }
+    };
+    Ring<NB> buf;
+    uint32_t loaded = 0, tiles = 0;
+    bool ok = true;
+    int index = blockIdx.x;
+    for (int it = 0; ok && index >= 0; ++it) {
+      const PromptPair r = prompt_pair(a, index);
+      if (r.n > 0) {
+        // the buffer of scores is free: the products before, which read the weights in it, have been issued before
+        ok = wait_warp(&kv_full[buf.at], buf.round & 1u);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ok = ok && wait_warp(&q_full[i], loaded & 1u);
+          if (ok && elect_one()) {
+            scores(i, buf.at);
+            if (i == 1) {
+              ptx::umma_commit(&kv_empty[buf.at]);
+              if (r.n == 1) ptx::umma_commit(&q_empty);
+            }
+          }
+          __syncwarp();
         }
-        if (ok && !(whole(0, first_key) && whole(1, first_key))) {
-          ok = wait_warp(&v_ok, guards & 1u);
-          ++guards;
+        ++loaded;
+        buf.next();
+      }
+      for (int j = 0; ok && j < r.n; ++j, ++tiles) {
+        const int vbuf = buf.at;
+        ok = wait_warp(&kv_full[vbuf], buf.round & 1u) && wait_warp(&v_ok[tiles % kChecks], (tiles / kChecks) & 1u);
+        buf.next();
+        const int kbuf = buf.at;
+        const bool more = j + 1 < r.n;
+        if (ok && more) {
+          ok = wait_warp(&kv_full[kbuf], buf.round & 1u);
+          buf.next();
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // the first half of the products starts while the second half of the weights is computed
-          ok = ok && wait_warp(&p_full[i][0], j & 1u);
+          ok = ok && wait_warp(&p_full[i][0], tiles & 1u);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           if (elect_one()) outputs(i, 0, vbuf, j == 0);
           __syncwarp();
-          ok = wait_warp(&p_full[i][1], j & 1u);
+          ok = wait_warp(&p_full[i][1], tiles & 1u);
           if (!ok) break;
           ptx::tc_fence_after_sync();
           if (elect_one()) {
@@ -388,15 +491,56 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
             if (i == 1) ptx::umma_commit(&kv_empty[vbuf]);
             if (more) {
               scores(i, kbuf);
-              if (i == 1) ptx::umma_commit(&kv_empty[kbuf]);
+              if (i == 1) {
+                ptx::umma_commit(&kv_empty[kbuf]);
+                if (j + 2 == r.n) ptx::umma_commit(&q_empty);
+              }
             }
           }
           __syncwarp();
         }
       }
+      if (ok) index = next_pair(it);
     }
   } else if (warp >= 10) {
     hand_over();
+    Ring<NB> buf;  // keys, values, keys, ...
+    uint32_t loaded = 0, tiles = 0;
+    bool ok = true;
+    int index = blockIdx.x;
+    for (int it = 0; ok && index >= 0; ++it) {
+      const PromptPair r = prompt_pair(a, index);
+      for (int j = 0; ok && j < r.n; ++j, ++tiles) {
+        const int first_key = r.tiles.start(j);
+        buf.next();
+        ok = wait_warp(&kv_full[buf.at], buf.round & 1u);
+        if (!ok) break;
+        if (!seen_by_all(a, r, first_key)) {
+          const uint32_t at = ring + buf.at * TILE + (threadIdx.x - 320) * 16;
+          const int here = r.length - first_key;  // tokens of the tile that the sequence has
+          uint32_t m = 0;
+          if (here < kTileKeys) {
+#pragma unroll 4
+            for (int x = 0; x < TILE; x += 64 * 16) {
+              if (((x + (threadIdx.x - 320) * 16) & (BLOCK - 1)) / 128 >= here) ptx::st_shared_v4(at + x, make_uint4(0, 0, 0, 0));
+            }
+          }
+#pragma unroll 8
+          for (int x = 0; x < TILE; x += 64 * 16) m = magnitudes(m, ptx::ld_shared_v4(at + x));
+          if (!all_finite<BF16>(m)) *const_cast<volatile int*>(&odd_pair[loaded & 1]) = static_cast<int>(loaded) + 1;
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        // (for every tile: the products do not start without it, so that this warp cannot fall behind the ring)
+        if (lane == 0) ptx::mbar_arrive(&v_ok[tiles % kChecks]);
+        buf.next();
+      }
+      if (ok && r.n > 0) {
+        if (lane == 0) ptx::mbar_arrive(&checked[loaded & 1]);
+        ++loaded;
+      }
+      if (ok) index = next_pair(it);
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     const int tile = warp >> 2;
@@ -404,172 +548,193 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes each, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * kTileKeys, t_o = tmem + lanes + 2 * kTileKeys + tile * 128;
     const int token = row / a.group, head = row - token * a.group;
-    const int t = blk.t0 + tile * a.tokens + token;
-    const int pos = p.sk - p.sq + t;
-    const bool real = token < a.tokens && t < p.sq;
-    const int last = real && pos < blk.length ? pos : -1;  // the last visible token
-    const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
     const float c = a.scale_log2;
-    float m = kLowest, l = 0.f;
+    uint32_t loaded = 0, tiles = 0;
     bool ok = true;
-    int vbuf = 1, guards = 0;
-    uint32_t vround = 0;
-    for (int j = 0; j < blk.n; ++j) {
-      const int first_key = blk.tiles.tile(j) * kTileKeys;
-      ok = wait_warp(&s_full[tile], j & 1u);
-      if (!ok) break;
-      ptx::tc_fence_after_sync();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32b_x32(t_s + q * 32, s[q]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) ptx::tmem_ld_wait_for(s[q]);
-      const bool masked = !whole(tile, first_key);
-      if (masked) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int k0 = first_key + q * 32;
-          hide(s[q], bit_range(lo - k0, last - k0) | bit_range(0, min(p.sinks - 1, last) - k0));
-        }
-      }
-      // (NaN counts as the largest: it makes all of its row NaN)
-      float top[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) top[q] = __uint_as_float(s[q][0]);
-#pragma unroll
-      for (int e = 1; e < 31; e += 2) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) top[q] = max3_nan(top[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
-      }
-      top[0] = max3_nan(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
-      top[1] = max3_nan(top[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
-      const float most = max3_nan(max3_nan(top[0], top[1], m), top[2], top[3]);
-      const bool raise = real && !((most - m) * c <= kRaise);  // also for NaN; rows that no token fills hold anything
-      if (__any_sync(0xffffffffu, raise)) {
-        const float factor = raise ? exp2_fast((m - most) * c) : 1.f;
-        if (raise) m = most;
-        l *= factor;
-        if (j > 0) {
-          // the products of the tile before must have arrived; the next ones wait for this tile's weights
-          ok = wait_warp(&o_done[tile], (j - 1) & 1u);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-#pragma unroll
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
-            ptx::tmem_ld_wait_for(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-            tmem_st_32x32b_x32(t_o + q * 32, o);
-          }
-          tmem_st_wait();
-        }
-      }
-      // A hidden token's weight is zero, and zero times infinity is not: tiles that are not seen whole have their values looked
-      // at (by both groups of warps, half of a tile each).  Tokens behind the length become zero; should any other be
-      // infinite or not a number, the rows of this CTA are computed one by one at the end.
-      if (masked || !whole(1 - tile, first_key)) {
-        ok = wait_warp(&kv_full[vbuf], vround & 1u);
+    int index = blockIdx.x;
+    for (int it = 0; index >= 0; ++it) {
+      const PromptPair r = prompt_pair(a, index);
+      const int t = r.t0 + tile * a.tokens + token;
+      const int pos = p.sk - p.sq + t;
+      const bool real = token < a.tokens && t < p.sq;
+      const int last = real && pos < r.length ? pos : -1;  // the last visible token
+      const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
+      float m = kLowest, l = 0.f;
+      for (int j = 0; j < r.n; ++j, ++tiles) {
+        const int first_key = r.tiles.start(j);
+        const bool masked = !sees_whole(a, r, tile, first_key);
+        ok = wait_warp(&s_full[tile], tiles & 1u);
         if (!ok) break;
-        bool odd = false;
-#pragma unroll 1
-        for (int x = threadIdx.x; x < TILE / 16; x += kSoftmaxThreads) {
-          const uint32_t at = ring + vbuf * TILE + x * 16;
-          if (first_key + (x & (BLOCK / 16 - 1)) / 8 >= blk.length) {
-            ptx::st_shared_v4(at, make_uint4(0, 0, 0, 0));
-          } else {
-            const uint4 v = ptx::ld_shared_v4(at);
-            odd = odd || pair_not_finite<BF16>(v.x) || pair_not_finite<BF16>(v.y) || pair_not_finite<BF16>(v.z) ||
-                  pair_not_finite<BF16>(v.w);
+        ptx::tc_fence_after_sync();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32b_x32(t_s + q * 32, s[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ptx::tmem_ld_wait_for(s[q]);
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int k0 = first_key + q * 32;
+            const uint32_t see = bit_range(lo - k0, last - k0) | bit_range(0, min(p.sinks - 1, last) - k0);
+            // rows of a tile are a few tokens apart: many words are full in all lanes
+            if (!__all_sync(0xffffffffu, see == 0xffffffffu)) hide(s[q], see);
           }
         }
-        if (odd) dirty = 1;
-        ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(&v_ok);
-        ++guards;
-      }
-      float base = m == kLowest ? 0.f : m * c;
-      base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
-      const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
-      Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
+        // (NaN counts as the largest: it makes all of its row NaN)
+        float top[4];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
+        for (int q = 0; q < 4; ++q) top[q] = __uint_as_float(s[q][0]);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
-          const Pair x = fma2(make_pair(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, base2);
-          float2 y;
-          if (e % kPolyEvery == kPolyEvery - 1) {
-            y = exp2_poly(x);
-          } else {
-            y = split(x);
-            y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+        for (int e = 1; e < 31; e += 2) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) top[q] = max3_nan(top[q], __uint_as_float(s[q][e]), __uint_as_float(s[q][e + 1]));
+        }
+        top[0] = max3_nan(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
+        top[1] = max3_nan(top[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
+        const float most = max3_nan(max3_nan(top[0], top[1], m), top[2], top[3]);
+        const bool raise = real && !((most - m) * c <= kRaise);  // also for NaN; rows that no token fills hold anything
+        if (__any_sync(0xffffffffu, raise)) {
+          const float factor = raise ? exp2_fast((m - most) * c) : 1.f;
+          if (raise) m = most;
+          l *= factor;
+          if (j > 0) {
+            // the products of the tile before must have arrived; the next ones wait for this tile's weights
+            ok = wait_warp(&o_done[tile], (tiles - 1) & 1u);
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
+              ptx::tmem_ld_wait_for(o);
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+              tmem_st_32x32b_x32(t_o + q * 32, o);
+            }
+            tmem_st_wait();
           }
-          sum[e & 1] = add2(sum[e & 1], make_pair(y.x, y.y));
-          w[e] = pack<BF16>(y.x, y.y);
         }
-        tmem_st_32x32b_x32(t_s + half * 32, w);
-        tmem_st_wait();
-        ptx::tc_fence_before_sync();
-        ptx::mbar_arrive(&p_full[tile][half]);
-      }
-      const float2 total = split(add2(sum[0], sum[1]));
-      l += total.x + total.y;
-      vbuf += 2;
-      if (vbuf >= NB) {
-        vbuf -= NB;
-        ++vround;
-      }
-    }
-    if (blk.n > 0 && ok) {
-      ok = wait_warp(&o_done[tile], (blk.n - 1) & 1u);
-      ptx::tc_fence_after_sync();
-    }
-    // everybody's findings are in: dirty, failed
-    ptx::named_barrier_sync(1, kSoftmaxThreads);
-    const bool by_rows = *const_cast<volatile int*>(&dirty) != 0, gave_up = *const_cast<volatile int*>(&failed) != 0;
-    uint16_t* dst = static_cast<uint16_t*>(p.out) +
-                    ((static_cast<long long>(blk.b) * p.sq + t) * p.heads + blk.kv_head * a.group + head) * D;
-    if (!by_rows || gave_up) {
-      const float inv = gave_up ? NAN : l == 0.f ? 0.f : 1.f / l;
+        float base = m == kLowest ? 0.f : m * c;
+        base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
+        const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
+        Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t o[32] = {};
-        if (blk.n > 0) {
-          ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
-          ptx::tmem_ld_wait_for(o);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
+            const Pair x = fma2(make_pair(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, base2);
+            float2 y;
+            if (e % kPolyEvery == kPolyEvery - 1) {
+              y = exp2_poly(x);
+            } else {
+              y = split(x);
+              y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            }
+            sum[e & 1] = add2(sum[e & 1], make_pair(y.x, y.y));
+            w[e] = pack<BF16>(y.x, y.y);
+          }
+          tmem_st_32x32b_x32(t_s + half * 32, w);
+          tmem_st_wait();
+          ptx::tc_fence_before_sync();
+          ptx::mbar_arrive(&p_full[tile][half]);
         }
-        if (real) {
-          // a row that sees nothing is zero, whatever its accumulator holds
+        const float2 total = split(add2(sum[0], sum[1]));
+        l += total.x + total.y;
+      }
+      bool by_rows = false;
+      if (ok && r.n > 0) {
+        ok = wait_warp(&checked[loaded & 1], (loaded >> 1) & 1u) && wait_warp(&o_done[tile], (tiles - 1) & 1u);
+        ptx::tc_fence_after_sync();
+        ++loaded;
+        by_rows = *const_cast<volatile int*>(&odd_pair[(loaded - 1) & 1]) == static_cast<int>(loaded);
+      }
+      if (!ok) {
+        if (lane == 0) atomicMin(&unfinished, it);
+        break;
+      }
+      if (!by_rows) {
+        // Through shared memory, so that a store instruction writes four whole lines and not parts of 32: a row's chunks of 16
+        // bytes go in where the row's number puts them, eight lanes read a row.
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const uint32_t out = stage + warp * kStageBytes;
+        const int chunk = lane & 7;
+        const long long mine =
+            real ? ((static_cast<long long>(r.b) * p.sq + t) * p.heads + r.kv_head * a.group + head) * D : -1;
+        long long to[8];  // the rows whose chunks this lane stores
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 8; ++e) to[e] = __shfl_sync(0xffffffffu, mine, e * 4 + (lane >> 3));
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) {
+          uint32_t o[2][32] = {};
+          if (r.n > 0) {
+            ptx::tmem_ld_32x32b_x32(t_o + x * 64, o[0]);
+            ptx::tmem_ld_32x32b_x32(t_o + x * 64 + 32, o[1]);
+            ptx::tmem_ld_wait_for(o[0]);
+            ptx::tmem_ld_wait_for(o[1]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
             uint32_t w[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float f0 = __uint_as_float(o[e * 8 + x * 2]), f1 = __uint_as_float(o[e * 8 + x * 2 + 1]);
-              w[x] = inv == 0.f ? 0u : pack<BF16>(f0 * inv, f1 * inv);
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t* src = o[e >> 2] + (e & 3) * 8 + y * 2;
+              // a row that sees nothing is zero, whatever its accumulator holds
+              w[y] = inv == 0.f ? 0u : pack<BF16>(__uint_as_float(src[0]) * inv, __uint_as_float(src[1]) * inv);
             }
-            ptx::st_v4(dst + q * 32 + e * 8, make_uint4(w[0], w[1], w[2], w[3]));
+            ptx::st_shared_v4(out + lane * 128 + ((e ^ (lane & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+          }
+          __syncwarp();
+          uint4 v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int from = e * 4 + (lane >> 3);
+            v[e] = ptx::ld_shared_v4(out + from * 128 + ((chunk ^ (from & 7)) << 4));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (to[e] >= 0) ptx::st_v4(static_cast<uint16_t*>(p.out) + to[e] + x * 64 + chunk * 8, v[e]);
           }
         }
+        ptx::tc_fence_before_sync();
+      } else {
+        for (int x = warp & 3; x < a.group * a.tokens; x += 4) {
+          const int tok = r.t0 + tile * a.tokens + x / a.group;
+          if (tok < p.sq) exact_row<D, BF16>(p, r.b, tok, r.kv_head * a.group + x % a.group, r.length, c);
+        }
       }
-    } else {
-      const int rows = a.group * a.tokens;
-      for (int r = warp; r < 2 * rows; r += kSoftmaxThreads / 32) {
-        const int tok = blk.t0 + r / a.group;
-        if (tok < p.sq) exact_row<D, BF16>(p, blk.b, tok, blk.kv_head * a.group + r % a.group, blk.length, c);
+      index = next_pair(it);
+      if (index < 0 && *const_cast<volatile int*>(&failed) != 0) {
+        if (lane == 0) atomicMin(&unfinished, it + 1);
       }
     }
-    ptx::tc_fence_before_sync();
   }
   __syncthreads();
-  if (failed != 0) {
-    // a wait ran out: copies and products that are still under way get time to end before their memory is given back
+  if (*const_cast<volatile int*>(&failed) != 0) {
+    // A wait ran out: copies, answers and products that are still under way get time to end before their memory is given
+    // back, and the rows of all pairs that this CTA has taken and not finished become NaN.
     const uint64_t until = ptx::globaltimer_ns() + 2000000ull;
     while (ptx::globaltimer_ns() < until) __nanosleep(1000);
     __syncthreads();
+    const int rows = 2 * a.tokens * a.group;
+    for (int it = unfinished; it <= taken; ++it) {
+      int index = -1;
+      if (it < taken) index = pairs[it & 3];
+      else if (pending >= 0 && ptx::mbar_try_wait(&next_full[pending & 1], (pending >> 1) & 1u)) index = claimed_cta(&answers[pending & 1]);
+      if (index < 0) continue;
+      const PromptPair r = prompt_pair(a, index);
+      for (int x = threadIdx.x; x < rows * (D / 8); x += kPromptThreads) {
+        const int y = x / (D / 8), t = r.t0 + y / a.group;
+        if (t < p.sq) {
+          ptx::st_v4(static_cast<uint16_t*>(p.out) +
+                         ((static_cast<long long>(r.b) * p.sq + t) * p.heads + r.kv_head * a.group + y % a.group) * D +
+                         (x % (D / 8)) * 8,
+                     make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu));
+        }
+      }
+    }
   }
   if (warp == 8) {
     ptx::tc_fence_after_sync();

@@ -61,17 +61,23 @@ def test_tiles_hold_all_visible_tokens_once(tile):
         p0 = rng.randrange(0, 900)
         p1 = p0 + rng.choice([0, 1, 31, 127])
         window, sinks = rng.choice([0, 1, 2, 63, 64, 65, 300, 2 ** 31 - 1]), rng.choice([0, 1, 4, 63, 64, 65, 500, 2 ** 31 - 1])
-        tiles = OPS.seen_tiles(p0, p1, length, window, sinks, tile)
-        assert len(set(tiles)) == len(tiles) and tiles == sorted(tiles)
-        need = {j // tile for i in range(p0, p1 + 1) for j in range(min(i + 1, length))
+        starts = OPS.seen_tiles(p0, p1, length, window, sinks, tile)
+        assert all(b - a >= tile for a, b in zip(starts, starts[1:])) and all(0 <= a < length for a in starts)
+        held = {j for a in starts for j in range(a, a + tile)}
+        need = {j for i in range(p0, p1 + 1) for j in range(min(i + 1, length))
                 if window == 0 or j > i - window or j < sinks}
-        assert need <= set(tiles)
-        # nothing beyond: every tile has a token that some position between sees, or lies between such tiles
-        if p0 == p1 and p1 < length:
-            assert need == set(tiles)
-        if not need:
-            assert len(tiles) == 0 or p0 >= length
-        assert all(0 <= t * tile < max(length, 1) for t in tiles)
+        assert need <= held
+        if p1 < length:     # no more tiles than the sinks and the rest take
+            lo = max(0, p0 - window + 1) if window else 0
+            front = min(sinks, lo)
+            assert len(starts) <= -(-front // tile) + -(-(p1 + 1 - lo) // tile)
+
+
+def test_tiles_of_the_longest_sequences():
+    top = 2 ** 31 - 1025
+    assert len(OPS.seen_tiles(top - 1, top - 1, top, 100, 2 ** 20, 64)) == 2 ** 14 + 2
+    assert OPS.seen_tiles(top - 1, top - 1, top, 100, 3, 64) == [0, top - 100, top - 36]
+    assert OPS.seen_tiles(top - 1, top - 1, top, 2 ** 31 - 1, 3, 1024)[0] == 0
 
 
 def test_operators_refuse_tensors_on_the_cpu():
