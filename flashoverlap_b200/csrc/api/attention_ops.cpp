@@ -330,12 +330,14 @@ static std::vector<int64_t> page_place_op(std::vector<int64_t> row, int64_t pos,
   return {page, place, page < 0 ? -1 : l.key_offset(page, static_cast<int>(head), place)};
 }
 // First tokens of the tiles of `tile` tokens that the positions [p0, p1] of a sequence look at, by the function the kernels use.
-static std::vector<int64_t> seen_tiles_op(int64_t p0, int64_t p1, int64_t length, int64_t window, int64_t sinks, int64_t tile) {
+static std::vector<int64_t> seen_tiles_op(int64_t p0, int64_t p1, int64_t length, int64_t window, int64_t sinks, int64_t tile,
+                                          int64_t align) {
   TORCH_CHECK(p0 >= -1 && p0 <= p1 && p1 < std::numeric_limits<int>::max() && length >= 0 &&
-                  length <= std::numeric_limits<int>::max() - 1024 && tile > 0 && tile <= 1024, "seen_tiles: bad arguments");
+                  length <= std::numeric_limits<int>::max() - 1024 && tile > 0 && tile <= 1024 && align > 0 && tile % align == 0, "seen_tiles: bad arguments");
   check_window(window, sinks);
   const SeenTiles t = seen_tiles(static_cast<int>(p0), static_cast<int>(p1), static_cast<int>(length),
-                                 static_cast<int>(window), static_cast<int>(sinks), static_cast<int>(tile));
+                                 static_cast<int>(window), static_cast<int>(sinks), static_cast<int>(tile),
+                                 static_cast<int>(align));
   std::vector<int64_t> out;
   for (int i = 0; i < t.count(); ++i) out.push_back(t.start(i));
   return out;

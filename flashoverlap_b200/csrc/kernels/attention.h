@@ -54,9 +54,9 @@ struct PageLayout {
     const int slot = static_cast<int>(by_page.div(static_cast<uint32_t>(pos)));
     place = pos - slot * page_size;
     if (slot >= width) return -1;
-    const int page = row[slot];
-    return page >= 0 && page < pages ? page : -1;
+    return has(row[slot]) ? row[slot] : -1;
   }
+  __host__ __device__ bool has(int page) const { return page >= 0 && page < pages; }
 };
 
 // Tiles of `tile` tokens: the first n_sink of the sequence, then n from token `first` on.
@@ -66,8 +66,9 @@ struct SeenTiles {
   __host__ __device__ int start(int i) const { return i < n_sink ? i * tile : first + (i - n_sink) * tile; }
 };
 // The tiles that hold the tokens which some position of [p0, p1] sees in a sequence of `length` tokens, p0 <= p1.  A window's
-// tiles begin with the first token it shows, wherever that is, and not at a multiple of the tile.
-__host__ __device__ inline SeenTiles seen_tiles(int p0, int p1, int length, int window, int sinks, int tile) {
+// tiles begin with the first token it shows, rounded down to a multiple of `align` (which divides `tile`), and not at a
+// multiple of the tile.
+__host__ __device__ inline SeenTiles seen_tiles(int p0, int p1, int length, int window, int sinks, int tile, int align) {
   SeenTiles t;
   const int end = p1 < length ? p1 + 1 : length;  // behind the last visible token
   // (p0 - window may be far below zero, never below the smallest int)
@@ -77,7 +78,8 @@ __host__ __device__ inline SeenTiles seen_tiles(int p0, int p1, int length, int 
   t.tile = tile;
   t.n_sink = sink > 0 ? (sink - 1) / tile + 1 : 0;
   const int behind = t.n_sink * tile;  // (below the largest int: a tile more than a length of at most 2^31 - 1024)
-  t.first = lo > behind ? lo : behind;
+  t.first = lo > behind ? lo - lo % align : behind;
+  if (t.first < behind) t.first = behind;
   t.n = end > t.first ? (end - t.first - 1) / tile + 1 : 0;
   return t;
 }

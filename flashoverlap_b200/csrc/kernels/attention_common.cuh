@@ -1,6 +1,10 @@
 // Device pieces that the attention kernels share: 16-bit conversions, asynchronous copies, warp matrix instructions.
 #pragma once
 
+#include <mutex>
+#include <set>
+#include <utility>
+
 #include "attention.h"
 #include "sm100_ptx.cuh"
 
@@ -85,6 +89,9 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take)
   const int n = take ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
@@ -104,6 +111,13 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "memory");
 }
 
+// An 8 x 8 matrix of 16-bit values, two of a row in each lane, the other way round.
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
 // d[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums.
 template <bool BF16>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -116,6 +130,22 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+}
+
+// Dynamic shared memory of a kernel, asked for once on each device.
+template <typename... Params>
+cudaError_t allow_smem(void (*kernel)(Params...), int bytes) {
+  static std::mutex mu;
+  static std::set<std::pair<int, const void*>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const std::pair<int, const void*> key(dev, reinterpret_cast<const void*>(kernel));
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count(key)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.insert(key);
+  return e;
 }
 
 // Launch whose CTAs may be placed while the kernel before it drains (they wait for it themselves).

@@ -1,8 +1,7 @@
 // Attention of one new token per sequence over a paged cache.
 //
 // With one query row per head the work is reading keys and values once: bound by HBM.  The query heads that share a key and
-// value head are the rows of a 16-row warp matrix product, so every byte read serves all of them; the tensor pipe is far
-// from its limit (two products of 16 x 16 x head_dim per 16 tokens), and rows that no head fills cost nothing that counts.
+// value head are the columns of warp matrix products whose rows are tokens, so every byte read serves all of them.
 //
 // The work is one line of tiles of 64 tokens: sequence by sequence, head by head, along the visible part of the length.  It
 // is cut into equal stretches, one per CTA, whatever the lengths are: one long sequence and a batch of ragged ones fill the
@@ -25,18 +24,27 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kStrip = 16;               // tokens of a warp
-constexpr int kTile = kWarps * kStrip;   // tokens of a CTA
-constexpr int kRows = 16;                // query heads that one pass serves
+constexpr int kRows = 16;      // query heads that one pass serves
 constexpr int kCtasPerSm = 2;
+constexpr int kStages = 3;     // of a warp's ring, 8 KB each (two CTAs then take all of an SM's shared memory)
 
+// Tokens of a warp and of a CTA.  8 KB of keys and values either way: with 16 tokens of 64 values, what a warp does for every
+// strip whatever its size (maxima, page numbers, the end of the loop) took longer than the data.
 template <int D>
-constexpr int stages() {
-  return D == 128 ? 3 : 4;
+constexpr int strip_tokens() {
+  return D == 128 ? 16 : 32;
+}
+template <int D>
+constexpr int tile_tokens() {
+  return kWarps * strip_tokens<D>();
 }
 template <int D>
 constexpr int strip_bytes() {
-  return kStrip * D * 2;
+  return strip_tokens<D>() * D * 2;
+}
+template <int D>
+constexpr int paged_smem_bytes() {
+  return kWarps * kStages * 2 * strip_bytes<D>() + kWarps * 8 * D * static_cast<int>(sizeof(float));
 }
 
 // Query heads of a key and value head are served `rows` at a time, in `subs` passes of their own.
@@ -51,19 +59,23 @@ HeadSplit head_split(const PagedParams& p) {
   return h;
 }
 
-// What the launch leaves for the joining kernel: {sequence, virtual head, slot of the first part, parts} for the CTA that
-// holds the second part of a stretch, {-1, ...} for all others.
+// What the launch leaves for the joining kernel.
 struct Partials {
   float* out;   // [2 * ctas][rows][D]: the first sequence of a CTA in slot 2 c, its last one in 2 c + 1
   float2* ml;   // [2 * ctas][rows]: largest score (times log2 e), sum of weights
-  int4* joins;  // [ctas]
+  // {sequence, virtual head, slot of the first part, parts}, -1: nothing to join.  One for each sequence and virtual head, or
+  // for each CTA (the one that holds the first part) where those are fewer.
+  int4* joins;
+  int by_unit;
 };
 
 struct PagedArgs {
   PagedParams p;
   HeadSplit h;
   Partials part;
+  // The scale is positive; a negative one has its sign in the queries, with a scale of zero they are zero.
   float scale_log2;
+  uint32_t q_and, q_xor;
 };
 
 // The tiles of one sequence.
@@ -72,18 +84,19 @@ struct Sequence {
   int length, count;
   bool bad;  // longer than its table
 };
-__device__ __forceinline__ Sequence sequence(const PagedParams& p, int s) {
+__device__ __forceinline__ Sequence sequence(const PagedParams& p, int s, int tile) {
   Sequence q;
   const long long room = static_cast<long long>(p.width) * p.pages.page_size;
   const int n = max(__ldg(p.lengths + s), 0);
   q.bad = n > room;
   q.length = q.bad ? static_cast<int>(room) : n;
-  q.t = seen_tiles(q.length - 1, q.length - 1, q.length, p.window, p.sinks, kTile);
+  q.t = seen_tiles(q.length - 1, q.length - 1, q.length, p.window, p.sinks, tile, tile / kWarps);
   q.count = max(q.t.count(), 1);  // an empty sequence has a tile as well, of which nothing is visible: its rows become zero
   return q;
 }
 
 // A place on the line of tiles.
+template <int TILE>
 struct Cursor {
   int s, head, i, left;  // sequence, virtual head, tile of the sequence, tiles to go in this CTA
   Sequence q;
@@ -95,17 +108,15 @@ struct Cursor {
     if (++head < heads) return;
     head = 0;
     ++s;
-    if (left > 0) q = sequence(p, s);
+    if (left > 0) q = sequence(p, s, TILE);
   }
 };
 
-template <int D, bool BF16>
+template <int D, int NT, bool BF16>  // NT: query heads of a pass, in eights
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(const __grid_constant__ PagedArgs a) {
-  constexpr int ST = stages<D>(), BYTES = strip_bytes<D>(), CH = D / 8;
+  constexpr int ST = kStages, BYTES = strip_bytes<D>(), CH = D / 8, TOK = strip_tokens<D>(), TILE = tile_tokens<D>();
   const PagedParams& p = a.p;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int scan[kWarps];
-  __shared__ int start[3];                       // sequence, tiles in front of it, all tiles
+  extern __shared__ __align__(256) uint8_t smem[];  // (rows of up to 256 bytes are addressed with exclusive ors)
   __shared__ float2 ml[kWarps][kRows];
   __shared__ unsigned bad_pages[kWarps][ST];
   ptx::wait_for_previous_kernel();
@@ -113,97 +124,103 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads = p.pages.kv_heads * a.h.subs;
 
-  // Where this CTA's stretch begins: a thread adds up the tiles of its share of the sequences.
-  int per;
-  Cursor ic;
+  // Where this CTA's stretch begins.  Every warp finds it by itself, 32 sequences at a time: no barrier, one trip to memory
+  // for up to 32 sequences.
+  int per, at_tile;  // tiles of a CTA; place on the line of the tile at the cursor
+  Cursor<TILE> ic;
   {
-    const int share = (p.seqs + kThreads - 1) / kThreads;
-    const int s0 = min(static_cast<int>(threadIdx.x) * share, p.seqs), s1 = min(s0 + share, p.seqs);
-    int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += sequence(p, s).count;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
+    int total = 0, mine = 0;
+    for (int s0 = 0; s0 < p.seqs; s0 += 32) {
+      mine = s0 + lane < p.seqs ? sequence(p, s0 + lane, TILE).count : 0;
+      total += mine;
     }
-    if (lane == 31) scan[warp] = sum;
-    __syncthreads();
-    int before = sum - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
+    total = __reduce_add_sync(0xffffffffu, total);
     total *= heads;
     per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
     const long long first = static_cast<long long>(blockIdx.x) * per;
-    if (threadIdx.x == 0) start[2] = total;
-    if (first >= static_cast<long long>(before) * heads && first < static_cast<long long>(before + mine) * heads) {
-      int s = s0, at = before;
-      for (int n; first >= static_cast<long long>(at + (n = sequence(p, s).count)) * heads; ++s) at += n;
-      start[0] = s;
-      start[1] = at;
-    }
-    __syncthreads();
     if (first >= total) {
-      if (threadIdx.x == 0) a.part.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      if (threadIdx.x == 0 && !a.part.by_unit) a.part.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
       return;
     }
-    ic.s = start[0];
-    ic.q = sequence(p, ic.s);
-    const int within = static_cast<int>(first) - start[1] * heads;
-    ic.head = within / ic.q.count;
-    ic.i = within - ic.head * ic.q.count;
-    ic.left = min(per, total - static_cast<int>(first));
-    if (threadIdx.x == 0) {
-      // the stretch that this CTA continues, if the CTA before it holds its beginning
-      int4 join = make_int4(-1, 0, 0, 0);
-      if (ic.i > 0) {
-        const int begin = static_cast<int>(first) - ic.i;
-        if (begin / per + 1 == static_cast<int>(blockIdx.x)) {
-          join = make_int4(ic.s, ic.head, 2 * (begin / per) + (begin % per != 0), (begin + ic.q.count - 1) / per - begin / per + 1);
-        }
+    at_tile = static_cast<int>(first);
+    int before = 0;
+    for (int s0 = 0;; s0 += 32) {
+      if (p.seqs > 32) mine = s0 + lane < p.seqs ? sequence(p, s0 + lane, TILE).count : 0;
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += x;
       }
-      a.part.joins[blockIdx.x] = join;
+      // the first sequence that ends behind the stretch's beginning
+      const unsigned ends = __ballot_sync(0xffffffffu, (before + sum) * heads > at_tile);
+      if (ends != 0) {
+        const int which = __ffs(ends) - 1;
+        ic.s = s0 + which;
+        ic.q = sequence(p, ic.s, TILE);
+        const int within = at_tile - (before + __shfl_sync(0xffffffffu, sum - mine, which)) * heads;
+        ic.head = within / ic.q.count;
+        ic.i = within - ic.head * ic.q.count;
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, sum, 31);
     }
+    ic.left = min(per, total - at_tile);
   }
-  Cursor cc = ic;
+  Cursor<TILE> cc = ic;
 
   const uint32_t ring = ptx::smem_u32(smem) + warp * (ST * 2 * BYTES);
-  float* join_buf = reinterpret_cast<float*>(smem + kWarps * ST * 2 * BYTES);  // [2][rows][D]
+  float* join_buf = reinterpret_cast<float*>(smem + kWarps * ST * 2 * BYTES);  // [warps][8][D]
   const uint16_t* cache = static_cast<const uint16_t*>(p.cache);
   const long long value_off = p.pages.value_offset();
 
-  // Loads run ahead; the page of a token is looked up one tile before its load.
-  int page = -1, place = 0;
-  bool bad = false;
+  // Loads run ahead, and the page of a lane's token is asked for one strip before its load: nothing here waits for it.
+  int page = 0, place = 0;
+  bool seen = false, listed = false;
   auto look_up = [&] {
-    page = -1;
-    bad = false;
+    seen = false;
     if (ic.left > 0) {
-      const int pos = ic.first_token() + warp * kStrip + (lane & (kStrip - 1));
-      if (is_visible(ic.q.length - 1, pos, ic.q.length, p.window, p.sinks)) {
-        page = p.pages.find(p.table + ic.s * p.table_stride, p.width, pos, place);
-        bad = page < 0;
-      }
+      const int pos = ic.first_token() + warp * TOK + (lane & (TOK - 1));
+      seen = is_visible(ic.q.length - 1, pos, ic.q.length, p.window, p.sinks);
+      const int slot = static_cast<int>(p.pages.by_page.div(static_cast<uint32_t>(pos)));
+      place = pos - slot * p.pages.page_size;
+      listed = seen && slot < p.width;
+      if (listed) page = __ldg(p.table + ic.s * p.table_stride + slot);
     }
   };
   auto issue = [&](int slot) {
     if (ic.left > 0) {
       const int kv_head = ic.head / a.h.subs;
       const uint32_t dst = ring + slot * (2 * BYTES);
-      const unsigned any_bad = __ballot_sync(0xffffffffu, bad);
+      const bool found = listed && p.pages.has(page);
+      const long long mine = found ? p.pages.key_offset(page, kv_head, place) : -1;
+      const unsigned any_bad = __ballot_sync(0xffffffffu, seen && !found);
       if (lane == 0) bad_pages[warp][slot] = any_bad | (ic.q.bad ? 1u : 0u);
+      // A strip that is seen whole and lies in one stretch of memory (pages of whole strips) needs one address; else each row's
+      // comes from the lane that looked its token up.
+      constexpr int ROWS = 32 / CH;  // of an instruction
+      const int row0 = lane / CH, ch = lane % CH;
+      const uint32_t to = dst + row0 * (D * 2) + ((ch ^ row0) << 4);
+      const long long begin = __shfl_sync(0xffffffffu, mine, 0);
+      if (__all_sync(0xffffffffu, found && mine == begin + (lane & (TOK - 1)) * D)) {
+        const uint16_t* src = cache + begin + row0 * D + ch * 8;
+        const uint16_t* src_v = src + value_off;
 #pragma unroll
-      for (int i = 0; i < kStrip * CH / 32; ++i) {
-        const int row = (i * 32 + lane) / CH, ch = lane % CH;
-        const int pg = __shfl_sync(0xffffffffu, page, row), pl = __shfl_sync(0xffffffffu, place, row);
-        const bool take = pg >= 0;
-        const uint16_t* src = cache + (take ? p.pages.key_offset(pg, kv_head, pl) + ch * 8 : 0);
-        const uint32_t to = dst + row * (D * 2) + ((ch ^ (row & 7)) << 4);
-        copy16(to, src, take);
-        copy16(to + BYTES, src + (take ? value_off : 0), take);
+        for (int i = 0; i < TOK / ROWS; ++i) {
+          const uint32_t at = (to ^ (((i * ROWS) & 7) << 4)) + i * ROWS * (D * 2);
+          copy16(at, src + i * ROWS * D);
+          copy16(at + BYTES, src_v + i * ROWS * D);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < TOK / ROWS; ++i) {
+          const long long off = __shfl_sync(0xffffffffu, mine, i * ROWS + row0);
+          const bool take = off >= 0;
+          const uint16_t* src = cache + (take ? off + ch * 8 : 0);
+          const uint32_t at = (to ^ (((i * ROWS) & 7) << 4)) + i * ROWS * (D * 2);
+          copy16(at, src, take);
+          copy16(at + BYTES, src + (take ? value_off : 0), take);
+        }
       }
       ic.advance(p, heads);
       look_up();
@@ -214,10 +231,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) issue(i);
 
+  // Tokens are the rows of the products and query heads their columns, eight at a time: S^T = K q^T, O^T += V^T P^T.  (The
+  // other way round up to eight heads would fill half of 16 rows.)
   const int gr = lane >> 2, gc = lane & 3;  // row and column pair of a fragment
-  uint32_t qf[D / 16][4];
-  float o[D / 8][4], m[2], l[2];
+  uint32_t qf[D / 16][NT][2];
+  float o[D / 16][NT][4], m[NT][2], l[NT][2];
   bool fresh = true, spoiled = false, whole_start = cc.i == 0, first_segment = true;
+  int4 join = make_int4(-1, 0, 0, 0);
   int slot = 0, next_slot = ST - 1;
   while (cc.left > 0) {
     const int kv_head = cc.head / a.h.subs, sub = cc.head - kv_head * a.h.subs;
@@ -226,17 +246,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     if (fresh) {
       const uint16_t* q = static_cast<const uint16_t*>(p.q) + cc.s * p.q_stride[0];
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + gr;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = gr + (e & 1) * 8, c = ks * 16 + (e >> 1) * 8 + gc * 2;
-          qf[ks][e] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(q + (head0 + r) * p.q_stride[1] + c)) : 0u;
+        for (int ks = 0; ks < D / 16; ++ks) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = ks * 16 + e * 8 + gc * 2;
+            qf[ks][nt][e] =
+                r < rows ? (__ldg(reinterpret_cast<const uint32_t*>(q + (head0 + r) * p.q_stride[1] + c)) & a.q_and) ^ a.q_xor : 0u;
+          }
         }
-      }
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+        for (int i = 0; i < D / 16; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+      }
       spoiled = false;
       fresh = false;
     }
@@ -246,179 +271,195 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     const uint32_t keys = ring + slot * (2 * BYTES), values = keys + BYTES;
     spoiled |= bad_pages[warp][slot] != 0;
 
-    // scores of 16 rows and 16 tokens
-    float c[2][4] = {};
+    float c[TOK / 16][NT][4];
+#pragma unroll
+    for (int t = 0; t < TOK / 16; ++t) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) c[t][nt][0] = c[t][nt][1] = c[t][nt][2] = c[t][nt][3] = 0.f;
+    }
     {
-      const int row = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;
+      const int row = lane & 15;
+      const uint32_t at = keys + row * (D * 2) + (((lane >> 4) ^ (row & 7)) << 4);
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t b[4];
-        ldmatrix_x4(b, keys + row * (D * 2) + (((ks * 2 + half) ^ (row & 7)) << 4));
-        mma_16x8x16<BF16>(c[0], qf[ks], b[0], b[1]);
-        mma_16x8x16<BF16>(c[1], qf[ks], b[2], b[3]);
+#pragma unroll
+        for (int t = 0; t < TOK / 16; ++t) {
+          uint32_t k[4];
+          ldmatrix_x4(k, (at ^ (ks << 5)) + t * 16 * (D * 2));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16x8x16<BF16>(c[t][nt], k, qf[ks][nt][0], qf[ks][nt][1]);
+        }
       }
     }
-    const int pos0 = cc.first_token() + warp * kStrip;
-    float top[2] = {m[0], m[1]};
+    const int pos0 = cc.first_token() + warp * TOK;
+    const int asks = cc.q.length - 1;  // the position that asks
+    if (pos0 + TOK > cc.q.length || (p.window > 0 && asks - pos0 >= p.window && pos0 + TOK > p.sinks)) {
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+      for (int t = 0; t < TOK / 16; ++t) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int pos = pos0 + nt * 8 + gc * 2 + (e & 1);
-        const bool see = is_visible(cc.q.length - 1, pos, cc.q.length, p.window, p.sinks);
-        c[nt][e] = see ? c[nt][e] * a.scale_log2 : -INFINITY;
-        top[e >> 1] = fmaxf(top[e >> 1], c[nt][e]);
+        for (int e = 0; e < 2; ++e) {
+          if (!is_visible(asks, pos0 + t * 16 + e * 8 + gr, cc.q.length, p.window, p.sinks)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) c[t][nt][e * 2] = c[t][nt][e * 2 + 1] = -INFINITY;
+          }
+        }
       }
     }
     bool raised = false;
-    float alpha[2];
+    float alpha[NT][2];
+    uint32_t pf[TOK / 16][NT][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      const float base = top[r] == -INFINITY ? 0.f : top[r];
-      alpha[r] = exp2_fast(m[r] - base);
-      raised |= top[r] != m[r];
-      m[r] = top[r];
-      l[r] *= alpha[r];
-      top[r] = base;
-    }
-    uint32_t pf[4];
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+      for (int x = 0; x < 2; ++x) {
+        float top = m[nt][x];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        c[nt][e] = exp2_fast(c[nt][e] - top[e >> 1]);
-        l[e >> 1] += c[nt][e];
+        for (int t = 0; t < TOK / 16; ++t) top = fmaxf(top, fmaxf(c[t][nt][x], c[t][nt][x + 2]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        // (scale_log2 is positive: the sign is in the queries)
+        const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+        alpha[nt][x] = exp2_fast(m[nt][x] * a.scale_log2 - base);
+        raised |= top != m[nt][x];
+        m[nt][x] = top;
+        l[nt][x] *= alpha[nt][x];
+#pragma unroll
+        for (int t = 0; t < TOK / 16; ++t) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& w = c[t][nt][e * 2 + x];
+            w = exp2_fast(w * a.scale_log2 - base);
+            l[nt][x] += w;
+          }
+        }
       }
       // weights are rounded to the type of the values, as the tensor cores take them; their sum is not
-      pf[nt * 2] = pack<BF16>(c[nt][0], c[nt][1]);
-      pf[nt * 2 + 1] = pack<BF16>(c[nt][2], c[nt][3]);
+#pragma unroll
+      for (int t = 0; t < TOK / 16; ++t) {
+        pf[t][nt][0] = transpose_8x8(pack<BF16>(c[t][nt][0], c[t][nt][1]));
+        pf[t][nt][1] = transpose_8x8(pack<BF16>(c[t][nt][2], c[t][nt][3]));
+      }
     }
     if (__any_sync(0xffffffffu, raised)) {
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= alpha[0];
-        o[i][1] *= alpha[0];
-        o[i][2] *= alpha[1];
-        o[i][3] *= alpha[1];
+      for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][nt][e] *= alpha[nt][e & 1];
+        }
       }
     }
     {
-      const int row = (lane & 7) + (((lane >> 3) & 1) << 3), half = lane >> 4;
+      const int row = (lane & 7) + ((lane >> 4) << 3);
+      const uint32_t at = values + row * (D * 2) + ((((lane >> 3) & 1) ^ (row & 7)) << 4);
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, values + row * (D * 2) + (((j * 2 + half) ^ (row & 7)) << 4));
-        mma_16x8x16<BF16>(o[2 * j], pf, b[0], b[1]);
-        mma_16x8x16<BF16>(o[2 * j + 1], pf, b[2], b[3]);
+      for (int t = 0; t < TOK / 16; ++t) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t v[4];
+          ldmatrix_x4_trans(v, (at ^ (i << 5)) + t * 16 * (D * 2));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_16x8x16<BF16>(o[i][nt], v, pf[t][nt][0], pf[t][nt][1]);
+        }
       }
     }
     slot = slot + 1 == ST ? 0 : slot + 1;
     next_slot = next_slot + 1 == ST ? 0 : next_slot + 1;
 
-    // The end of a sequence and head, or of the CTA's stretch: the warps join.
+    // The end of a sequence and head, or of the CTA's stretch: the warps join, eight rows at a time.
     const bool whole_end = cc.i == cc.q.count - 1;
     if (whole_end || cc.left == 1) {
+      const bool whole = whole_start && whole_end;
+      const long long part = 2ll * blockIdx.x + (first_segment ? 0 : 1);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        if (spoiled) l[r] = NAN;
-        if (gc == 0) ml[warp][gr + r * 8] = make_float2(m[r], l[r]);
-      }
-      __syncthreads();
-      float scale[2], most[2], sum[2];
+      for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        most[r] = -INFINITY;
-        sum[r] = 0.f;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) most[r] = fmaxf(most[r], ml[w][gr + r * 8].x);
-        const float base = most[r] == -INFINITY ? 0.f : most[r];
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) sum[r] += ml[w][gr + r * 8].y * exp2_fast(ml[w][gr + r * 8].x - base);
-        scale[r] = exp2_fast(m[r] - base);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        o[i][0] *= scale[0];
-        o[i][1] *= scale[0];
-        o[i][2] *= scale[1];
-        o[i][3] *= scale[1];
-      }
-      auto at = [&](int which, int r, int i) {
-        return reinterpret_cast<float2*>(join_buf + (which * a.h.rows + gr + r * 8) * D + i * 8 + gc * 2);
-      };
-      auto put = [&](int which) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          if (gr < rows) *at(which, 0, i) = make_float2(o[i][0], o[i][1]);
-          if (gr + 8 < rows) *at(which, 1, i) = make_float2(o[i][2], o[i][3]);
+        for (int x = 0; x < 2; ++x) {
+          l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 4);
+          l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 8);
+          l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], 16);
+          if (spoiled) l[nt][x] = NAN;
+          if (gr == 0) ml[warp][nt * 8 + gc * 2 + x] = make_float2(m[nt][x] * a.scale_log2, l[nt][x]);
         }
-      };
-      auto add = [&](int which) {
+      }
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          if (gr < rows) {
-            const float2 x = *at(which, 0, i);
-            o[i][0] += x.x;
-            o[i][1] += x.y;
-          }
-          if (gr + 8 < rows) {
-            const float2 x = *at(which, 1, i);
-            o[i][2] += x.x;
-            o[i][3] += x.y;
-          }
-        }
-      };
-      if (warp >= 2) put(warp - 2);
-      __syncthreads();
-      if (warp < 2) add(warp);
-      if (warp == 1) put(1);
-      __syncthreads();
-      if (warp == 0) {
-        add(1);
-        if (whole_start && whole_end) {
+      for (int r = 0; r < NT; ++r) {
+        const int rows_here = min(rows - r * 8, 8);
+        if (rows_here > 0) {
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (gr + r * 8 < rows) {
+          for (int x = 0; x < 2; ++x) {
+            const int row = gc * 2 + x;
+            if (row < rows_here) {  // (columns exchanged so that rows begin in different banks)
+              float* to = join_buf + (warp * 8 + row) * D;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                to[(i * 16 + gr) ^ (gc << 3)] = o[i][r][x];
+                to[(i * 16 + 8 + gr) ^ (gc << 3)] = o[i][r][x + 2];
+              }
+            }
+          }
+          __syncthreads();
+          for (int x = threadIdx.x; x < rows_here * (D / 4); x += kThreads) {
+            const int row = x / (D / 4), col = (x - row * (D / 4)) * 4;
+            float most = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) most = fmaxf(most, ml[w][row + r * 8].x);
+            const float base = most == -INFINITY ? 0.f : most;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              const float2 its = ml[w][row + r * 8];
+              const float scale = exp2_fast(its.x - base);
+              const float4 z = *reinterpret_cast<const float4*>(join_buf + (w * 8 + row) * D + (col ^ ((row >> 1) << 3)));
+              sum += its.y * scale;
+              y.x += z.x * scale;
+              y.y += z.y * scale;
+              y.z += z.z * scale;
+              y.w += z.w * scale;
+            }
+            if (whole) {
               // nothing visible: zero.  (A sum that is not a number stays one.)
-              const float inv = sum[r] == 0.f ? 0.f : 1.f / sum[r];
-              uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) +
-                                                          (static_cast<long long>(cc.s) * p.heads + head0 + gr + r * 8) * D) + gc;
-#pragma unroll
-              for (int i = 0; i < D / 8; ++i) dst[i * 4] = pack<BF16>(o[i][r * 2] * inv, o[i][r * 2 + 1] * inv);
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p.out) +
+                                        (static_cast<long long>(cc.s) * p.heads + head0 + r * 8 + row) * D + col) =
+                  make_uint2(pack<BF16>(y.x * inv, y.y * inv), pack<BF16>(y.z * inv, y.w * inv));
+            } else {
+              const long long to = part * a.h.rows + r * 8 + row;
+              *reinterpret_cast<float4*>(a.part.out + to * D + col) = y;
+              if (col == 0) a.part.ml[to] = make_float2(most, sum);
             }
           }
-        } else {
-          const long long part = 2ll * blockIdx.x + (first_segment ? 0 : 1);
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if (gr + r * 8 < rows) {
-              const long long row = part * a.h.rows + gr + r * 8;
-              if (gc == 0) a.part.ml[row] = make_float2(most[r], sum[r]);
-              float2* dst = reinterpret_cast<float2*>(a.part.out + row * D) + gc;
-#pragma unroll
-              for (int i = 0; i < D / 8; ++i) dst[i * 4] = make_float2(o[i][r * 2], o[i][r * 2 + 1]);
-            }
-          }
+          __syncthreads();
         }
+      }
+      if (whole_start) {
+        const int begin = at_tile - cc.i;  // first tile of this sequence and head
+        const int4 mine = whole_end ? make_int4(-1, 0, 0, 0)
+                                    : make_int4(cc.s, cc.head, static_cast<int>(part),
+                                                (begin + cc.q.count - 1) / per - static_cast<int>(blockIdx.x) + 1);
+        if (!whole_end) join = mine;
+        if (a.part.by_unit && threadIdx.x == 0) a.part.joins[cc.s * heads + cc.head] = mine;
       }
       fresh = true;
       whole_start = true;
       first_segment = false;
     }
+    ++at_tile;
     cc.advance(p, heads);
   }
+  if (!a.part.by_unit && threadIdx.x == 0) a.part.joins[blockIdx.x] = join;
 }
 
-// Joins the parts of one stretch and one query head (blockIdx.y): warps take parts in turn, lanes take columns.
+// Joins the parts of one sequence and query head (blockIdx.y): warps take parts in turn, lanes take columns.
+constexpr int kJoinWarps = 16;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ PagedArgs a) {
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int V = D / 32;
-  __shared__ float red[kWarps][D];
-  __shared__ float2 sums[kWarps];
+  __shared__ float red[kJoinWarps][D];
+  __shared__ float2 sums[kJoinWarps];
   ptx::wait_for_previous_kernel();
   ptx::allow_next_kernel();
   const int4 join = a.part.joins[blockIdx.x];
@@ -428,45 +469,68 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   if (r >= min(a.h.rows, a.h.group - sub * a.h.rows)) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto row_of = [&](int i) {
-    const long long slot = i == 0 ? join.z : 2ll * (static_cast<int>(blockIdx.x) + i - 1);
+    const long long slot = i == 0 ? join.z : 2ll * ((join.z >> 1) + i);
     return slot * a.h.rows + r;
   };
-  float most = -INFINITY;
-  for (int i = lane; i < join.w; i += 32) most = fmaxf(most, a.part.ml[row_of(i)].x);
+  // kBatch parts in flight, with a running largest score
+  constexpr int kBatch = 8;
+  float acc[V] = {}, sum = 0.f, most = -INFINITY;
+  for (int i0 = warp; i0 < join.w; i0 += kJoinWarps * kBatch) {
+    float2 ml[kBatch];
+    float x[kBatch][V];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const float base = most == -INFINITY ? 0.f : most;
-  float acc[V] = {}, sum = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < join.w; i += kWarps) {
-    const long long row = row_of(i);
-    const float2 ml = a.part.ml[row];
-    const float w = exp2_fast(ml.x - base);
-    sum += ml.y * w;
-    const float* src = a.part.out + row * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(src);
-      acc[0] += x.x * w;
-      acc[1] += x.y * w;
-      acc[2] += x.z * w;
-      acc[3] += x.w * w;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(src);
-      acc[0] += x.x * w;
-      acc[1] += x.y * w;
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      const long long row = row_of(min(i, join.w - 1));
+      ml[k] = a.part.ml[row];
+      const float* src = a.part.out + row * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(src);
+        x[k][0] = y.x;
+        x[k][1] = y.y;
+        x[k][2] = y.z;
+        x[k][3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(src);
+        x[k][0] = y.x;
+        x[k][1] = y.y;
+      }
+      if (i >= join.w) ml[k] = make_float2(-INFINITY, 0.f);
+    }
+    float top = most;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float old = exp2_fast(most - base);
+    most = top;
+    sum *= old;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= old;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w = exp2_fast(ml[k].x - base);
+      sum += ml[k].y * w;
+      // (a part of weight zero adds nothing, also where it is not a number: its sum is then not one either)
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += x[k][v] * w;
     }
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) red[warp][lane * V + v] = acc[v];
-  if (lane == 0) sums[warp].x = sum;
+  if (lane == 0) sums[warp] = make_float2(most, sum);
   __syncthreads();
   if (threadIdx.x < D / 2) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sums[w].x);
+    const float base = top == -INFINITY ? 0.f : top;
     float total = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      total += sums[w].x;
-      x += red[w][threadIdx.x * 2];
-      y += red[w][threadIdx.x * 2 + 1];
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float scale = exp2_fast(sums[w].x - base);
+      total += sums[w].y * scale;
+      x += red[w][threadIdx.x * 2] * scale;
+      y += red[w][threadIdx.x * 2 + 1] * scale;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const int head = kv_head * a.h.group + sub * a.h.rows + r;
@@ -477,9 +541,14 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
 
 // CTAs of a launch: all that fit the chip together, but no more than there can be tiles.
 int grid_size(const PagedParams& p) {
+  const int tile = p.pages.head_dim == 128 ? tile_tokens<128>() : tile_tokens<64>();
   const long long tiles = static_cast<long long>(p.seqs) * p.pages.kv_heads * head_split(p).subs *
-                          std::max<long long>(1, (static_cast<long long>(p.width) * p.pages.page_size + kTile - 1) / kTile);
+                          std::max<long long>(1, (static_cast<long long>(p.width) * p.pages.page_size + tile - 1) / tile);
   return static_cast<int>(std::min<long long>(tiles, static_cast<long long>(kCtasPerSm) * device_sm_count()));
+}
+// Sequences and virtual heads.
+long long unit_count(const PagedParams& p) {
+  return static_cast<long long>(p.seqs) * p.pages.kv_heads * head_split(p).subs;
 }
 
 template <int D, bool BF16>
@@ -487,7 +556,9 @@ cudaError_t launch_typed(const PagedParams& p, cudaStream_t stream) {
   PagedArgs a;
   a.p = p;
   a.h = head_split(p);
-  a.scale_log2 = p.scale * kLog2e;
+  a.scale_log2 = p.scale == 0.f ? 1.f : std::fabs(p.scale) * kLog2e;
+  a.q_and = p.scale == 0.f ? 0u : ~0u;
+  a.q_xor = p.scale < 0.f ? 0x80008000u : 0u;
   const int grid = grid_size(p);
   char* ws = static_cast<char*>(p.workspace);
   a.part.out = reinterpret_cast<float*>(ws);
@@ -495,15 +566,15 @@ cudaError_t launch_typed(const PagedParams& p, cudaStream_t stream) {
   a.part.ml = reinterpret_cast<float2*>(ws);
   ws += (sizeof(float2) * 2 * grid * a.h.rows + 15) / 16 * 16;
   a.part.joins = reinterpret_cast<int4*>(ws);
-  constexpr int ring = kWarps * stages<D>() * 2 * strip_bytes<D>();
-  const size_t smem = ring + sizeof(float) * 2 * a.h.rows * D;
-  // (set for every launch: it belongs to the device that is current)
-  cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       ring + static_cast<int>(sizeof(float)) * 2 * kRows * D);
+  const long long units = unit_count(p);
+  a.part.by_unit = units < grid;
+  const auto kernel = a.h.rows <= 8 ? paged_attention_kernel<D, 1, BF16> : paged_attention_kernel<D, 2, BF16>;
+  cudaError_t e = allow_smem(kernel, paged_smem_bytes<D>());
   if (e != cudaSuccess) return e;
-  e = launch_after(paged_attention_kernel<D, BF16>, dim3(grid), kThreads, smem, stream, a);
+  e = launch_after(kernel, dim3(grid), kThreads, paged_smem_bytes<D>(), stream, a);
   if (e != cudaSuccess || grid == 1) return e;
-  return launch_after(join_kernel<D, BF16>, dim3(grid, a.h.rows), kThreads, 0, stream, a);
+  return launch_after(join_kernel<D, BF16>, dim3(static_cast<unsigned>(std::min<long long>(units, grid)), a.h.rows), kJoinWarps * 32,
+                      0, stream, a);
 }
 
 }  // namespace

@@ -221,7 +221,7 @@ __device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index
   r.t0 = (a.blocks - 1 - qb) * 2 * a.tokens;
   r.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + r.b), 0), p.sk);
   const int p0 = p.sk - p.sq + r.t0, p1 = p.sk - p.sq + min(r.t0 + 2 * a.tokens, p.sq) - 1;
-  r.tiles = seen_tiles(p0, p1, r.length, p.window, p.sinks, kTileKeys);
+  r.tiles = seen_tiles(p0, p1, r.length, p.window, p.sinks, kTileKeys, 1);
   r.n = p0 < r.length ? r.tiles.count() : 0;
   return r;
 }
@@ -806,8 +806,7 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   }
   const long long grid = static_cast<long long>(a.blocks) * p.batch * p.kv_heads;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(prompt_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       prompt_smem_bytes<D>());
+  cudaError_t e = allow_smem(prompt_attention_kernel<D, BF16>, prompt_smem_bytes<D>());
   if (e != cudaSuccess) return e;
   return launch_after(prompt_attention_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), kPromptThreads,
                       prompt_smem_bytes<D>(), stream, a);

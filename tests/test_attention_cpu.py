@@ -53,15 +53,15 @@ def test_division_by_the_page_size_is_exact():
             assert got[1] == pos % page, (page, pos)
 
 
-@pytest.mark.parametrize("tile", [16, 64, 128])
-def test_tiles_hold_all_visible_tokens_once(tile):
+@pytest.mark.parametrize("tile,align", [(16, 1), (64, 16), (128, 32), (128, 1), (64, 64)])
+def test_tiles_hold_all_visible_tokens_once(tile, align):
     rng = random.Random(tile)
     for _ in range(2000):
         length = rng.choice([0, 1, rng.randrange(1, 40), rng.randrange(1, 900)])
         p0 = rng.randrange(0, 900)
         p1 = p0 + rng.choice([0, 1, 31, 127])
         window, sinks = rng.choice([0, 1, 2, 63, 64, 65, 300, 2 ** 31 - 1]), rng.choice([0, 1, 4, 63, 64, 65, 500, 2 ** 31 - 1])
-        starts = OPS.seen_tiles(p0, p1, length, window, sinks, tile)
+        starts = OPS.seen_tiles(p0, p1, length, window, sinks, tile, align)
         assert all(b - a >= tile for a, b in zip(starts, starts[1:])) and all(0 <= a < length for a in starts)
         held = {j for a in starts for j in range(a, a + tile)}
         need = {j for i in range(p0, p1 + 1) for j in range(min(i + 1, length))
@@ -70,14 +70,15 @@ def test_tiles_hold_all_visible_tokens_once(tile):
         if p1 < length:     # no more tiles than the sinks and the rest take
             lo = max(0, p0 - window + 1) if window else 0
             front = min(sinks, lo)
-            assert len(starts) <= -(-front // tile) + -(-(p1 + 1 - lo) // tile)
+            assert len(starts) <= -(-front // tile) + -(-(p1 + 1 - lo // align * align) // tile)
+        assert all(a % align == 0 or a % tile == 0 for a in starts)
 
 
 def test_tiles_of_the_longest_sequences():
     top = 2 ** 31 - 1025
-    assert len(OPS.seen_tiles(top - 1, top - 1, top, 100, 2 ** 20, 64)) == 2 ** 14 + 2
-    assert OPS.seen_tiles(top - 1, top - 1, top, 100, 3, 64) == [0, top - 100, top - 36]
-    assert OPS.seen_tiles(top - 1, top - 1, top, 2 ** 31 - 1, 3, 1024)[0] == 0
+    assert len(OPS.seen_tiles(top - 1, top - 1, top, 100, 2 ** 20, 64, 1)) == 2 ** 14 + 2
+    assert OPS.seen_tiles(top - 1, top - 1, top, 100, 3, 64, 1) == [0, top - 100, top - 36]
+    assert OPS.seen_tiles(top - 1, top - 1, top, 2 ** 31 - 1, 3, 1024, 1)[0] == 0
 
 
 def test_operators_refuse_tensors_on_the_cpu():
