@@ -208,8 +208,11 @@ static void paged_attention_op(at::Tensor q, at::Tensor cache, at::Tensor page_t
   if (seqs == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
   // from the caching allocator, for this call alone: calls on other streams and captured graphs have their own
-  at::Tensor workspace = at::empty({static_cast<int64_t>(paged_workspace_bytes(p))}, q.options().dtype(at::kByte));
-  p.workspace = workspace.data_ptr();
+  at::Tensor workspace;
+  if (const size_t bytes = paged_workspace_bytes(p)) {
+    workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    p.workspace = workspace.data_ptr();
+  }
   check_launch(launch_paged_attention(p, dtype_of(q), at::cuda::getCurrentCUDAStream().stream()), "paged_attention");
 }
 

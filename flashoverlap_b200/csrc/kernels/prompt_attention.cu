@@ -783,7 +783,7 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   if (!fits_tiles(p)) {
     const long long rows = static_cast<long long>(p.batch) * p.sq * p.heads;
     const long long grid = std::min<long long>((rows + 7) / 8, 8ll * device_sm_count());
-    return launch_after(prompt_rows_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, p);
+    return launch_after(prompt_rows_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, 1, p);
   }
   PromptArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -809,7 +809,7 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   cudaError_t e = allow_smem(prompt_attention_kernel<D, BF16>, prompt_smem_bytes<D>());
   if (e != cudaSuccess) return e;
   return launch_after(prompt_attention_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), kPromptThreads,
-                      prompt_smem_bytes<D>(), stream, a);
+                      prompt_smem_bytes<D>(), stream, 1, a);
 }
 
 }  // namespace
