@@ -267,39 +267,45 @@ static void cache_append_op(at::Tensor k, at::Tensor v, at::Tensor cache, at::Te
 
 // moves [n, 2] on the CPU: page moves[i][0] of `cache` is copied to page moves[i][1].  Any tensor whose entries along the
 // first dimension are contiguous is a cache here.
-static void check_moves(const at::Tensor& moves, int64_t pages, std::vector<int>& list) {
-  TORCH_CHECK(moves.device().is_cpu(), "moves must be a CPU tensor");
-  TORCH_CHECK(moves.scalar_type() == at::kInt || moves.scalar_type() == at::kLong, "moves must be int32 or int64");
-  TORCH_CHECK(moves.dim() == 2 && moves.size(1) == 2, "moves must be [n, 2]: from page, to page");
-  const at::Tensor m = moves.to(at::kLong).contiguous();
-  const int64_t* at = m.data_ptr<int64_t>();
-  const int64_t n = m.size(0);
+template <typename Int>
+static void read_moves(const at::Tensor& moves, int64_t pages, std::vector<int>& list) {
+  const Int* at = moves.const_data_ptr<Int>();
+  const int64_t n = moves.size(0), row = moves.stride(0), col = moves.stride(1);
   list.resize(static_cast<size_t>(2 * n));
   std::vector<bool> target(static_cast<size_t>(pages), false);
   for (int64_t i = 0; i < n; ++i) {
     for (int64_t e = 0; e < 2; ++e) {
-      const int64_t page = at[2 * i + e];
+      const int64_t page = at[i * row + e * col];
       TORCH_CHECK(page >= 0 && page < pages, "moves names page ", page, ", outside [0, ", pages, ")");
       list[static_cast<size_t>(2 * i + e)] = static_cast<int>(page);
     }
-    const size_t to = static_cast<size_t>(at[2 * i + 1]);
+    const size_t to = static_cast<size_t>(list[static_cast<size_t>(2 * i + 1)]);
     TORCH_CHECK(!target[to], "moves writes page ", to, " twice");
     target[to] = true;
   }
   for (int64_t i = 0; i < n; ++i) {
-    TORCH_CHECK(!target[static_cast<size_t>(at[2 * i])], "moves reads page ", at[2 * i], " and writes it");
+    const size_t from = static_cast<size_t>(list[static_cast<size_t>(2 * i)]);
+    TORCH_CHECK(!target[from], "moves reads page ", from, " and writes it");
   }
 }
 static void copy_pages_op(at::Tensor cache, at::Tensor moves) {
   TORCH_CHECK(cache.dim() >= 1 && cache.size(0) <= std::numeric_limits<int>::max(), "cache must have pages");
+  TORCH_CHECK(moves.device().is_cpu(), "moves must be a CPU tensor");
+  TORCH_CHECK(moves.scalar_type() == at::kInt || moves.scalar_type() == at::kLong, "moves must be int32 or int64");
+  TORCH_CHECK(moves.dim() == 2 && moves.size(1) == 2, "moves must be [n, 2]: from page, to page");
   std::vector<int> list;
-  check_moves(moves, cache.size(0), list);
+  if (moves.scalar_type() == at::kInt) read_moves<int>(moves, cache.size(0), list);
+  else read_moves<int64_t>(moves, cache.size(0), list);
   TORCH_CHECK(cache.is_cuda(), "cache must be a CUDA tensor");
   TORCH_CHECK(!(at::GradMode::is_enabled() && cache.requires_grad()), "cache requires a gradient");
   if (list.empty()) return;
-  TORCH_CHECK(cache[0].is_contiguous(), "cache: a page must be contiguous");
+  int64_t values = 1;
+  for (int64_t d = cache.dim() - 1; d >= 1; --d) {
+    TORCH_CHECK(cache.size(d) == 1 || cache.stride(d) == values, "cache: a page must be contiguous");
+    values *= cache.size(d);
+  }
   const int64_t size = static_cast<int64_t>(cache.element_size());
-  const int64_t bytes = cache[0].numel() * size, stride = cache.size(0) > 1 ? cache.stride(0) * size : bytes;
+  const int64_t bytes = values * size, stride = cache.size(0) > 1 ? cache.stride(0) * size : bytes;
   if (bytes == 0) return;
   TORCH_CHECK(stride >= bytes, "cache: pages must not overlap");
   TORCH_CHECK(bytes % 16 == 0 && stride % 16 == 0 && reinterpret_cast<uintptr_t>(cache.data_ptr()) % 16 == 0,

@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
     for (long long t0 = static_cast<long long>(blockIdx.x) * rows + row; t0 < total; t0 += step * kTokensInFlight) {
       uint4 v[kTokensInFlight];
       long long to[kTokensInFlight];
+      // (the page is looked up while the token is on its way)
 #pragma unroll
       for (int u = 0; u < kTokensInFlight; ++u) {
         const long long t = t0 + u * step;
@@ -57,15 +58,12 @@ __global__ void __launch_bounds__(kThreads) cache_append_kernel(const __grid_con
         if (t < total) {
           const int s = static_cast<int>(by_tokens.div(static_cast<uint32_t>(t)));
           const int i = static_cast<int>(t - static_cast<long long>(s) * p.tokens);
-          const int start = __ldg(p.starts + s);
-          const bool wanted = (p.counts == nullptr || i < __ldg(p.counts + s)) && start >= 0 && start <= INT32_MAX - i;
-          if (wanted) {
+          if (p.counts == nullptr || i < __ldg(p.counts + s)) {
+            v[u] = __ldg(reinterpret_cast<const uint4*>(src + s * seq_stride + i * tok_stride));
+            const int start = __ldg(p.starts + s);
             int place;
-            const int page = p.pages.find(p.table + s * p.table_stride, p.width, start + i, place);
-            if (page >= 0) {
-              to[u] = p.pages.key_offset(page, head, place);
-              v[u] = __ldg(reinterpret_cast<const uint4*>(src + s * seq_stride + i * tok_stride));
-            }
+            const int page = start >= 0 && start <= INT32_MAX - i ? p.pages.find(p.table + s * p.table_stride, p.width, start + i, place) : -1;
+            if (page >= 0) to[u] = p.pages.key_offset(page, head, place);
           }
         }
       }
@@ -136,7 +134,7 @@ cudaError_t launch_cache_append(const AppendParams& p, cudaStream_t stream) {
 
 cudaError_t launch_copy_pages(void* cache, long long page_bytes, long long page_stride_bytes, const int* moves, int n,
                               cudaStream_t stream) {
-  constexpr int kFew = 480, kMany = 4000;  // 4 KB and 32 KB of launch parameters, the most that older and newer drivers take
+  constexpr int kFew = 60, kSome = 480, kMany = 4000;  // launch parameters of 512 bytes, 4 KB and 32 KB (the most there can be)
   if (page_bytes <= 0 || page_bytes % 16 != 0 || page_stride_bytes % 16 != 0) return cudaErrorInvalidValue;
   const long long chunks = page_bytes / 16;
   if (chunks >= (1ll << 30)) return cudaErrorInvalidValue;
@@ -144,9 +142,8 @@ cudaError_t launch_copy_pages(void* cache, long long page_bytes, long long page_
   const int most = static_cast<int>(std::min<long long>(kMany, std::max<long long>(1, (1ll << 30) / chunks)));
   for (int at = 0; at < n;) {
     const int some = std::min(n - at, most);
-    const cudaError_t e = some <= kFew
-                              ? copy_some<kFew>(static_cast<char*>(cache), chunks, page_stride_bytes, moves + 2 * at, some, stream)
-                              : copy_some<kMany>(static_cast<char*>(cache), chunks, page_stride_bytes, moves + 2 * at, some, stream);
+    const auto copy = some <= kFew ? copy_some<kFew> : some <= kSome ? copy_some<kSome> : copy_some<kMany>;
+    const cudaError_t e = copy(static_cast<char*>(cache), chunks, page_stride_bytes, moves + 2 * at, some, stream);
     if (e != cudaSuccess) return e;
     at += some;
   }
