@@ -156,6 +156,12 @@ static void prompt_attention_op(at::Tensor q, at::Tensor k, at::Tensor v, at::Te
   p.sinks = static_cast<int>(sinks);
   p.scale = scale_or(scale, dim);
   c10::cuda::CUDAGuard guard(q.device());
+  // from the caching allocator, for this call alone: calls on other streams and captured graphs have their own
+  at::Tensor workspace;
+  if (const size_t bytes = prompt_workspace_bytes(p)) {
+    workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+    p.workspace = workspace.data_ptr();
+  }
   check_launch(launch_prompt_attention(p, dtype_of(q), at::cuda::getCurrentCUDAStream().stream()), "prompt_attention");
 }
 
@@ -207,8 +213,7 @@ static void paged_attention_op(at::Tensor q, at::Tensor cache, at::Tensor page_t
   p.scale = scale_or(scale, dim);
   if (seqs == 0) return;
   c10::cuda::CUDAGuard guard(q.device());
-  // from the caching allocator, for this call alone: calls on other streams and captured graphs have their own
-  at::Tensor workspace;
+  at::Tensor workspace;  // as above
   if (const size_t bytes = paged_workspace_bytes(p)) {
     workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
     p.workspace = workspace.data_ptr();

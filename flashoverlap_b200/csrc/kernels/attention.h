@@ -95,7 +95,9 @@ struct PromptParams {
   int batch, sq, sk, heads, kv_heads, head_dim;
   int window, sinks;
   float scale;
+  void* workspace;  // prompt_workspace_bytes(), 16-byte aligned, contents arbitrary
 };
+size_t prompt_workspace_bytes(const PromptParams& p);
 // head_dim 64 or 128, heads a multiple of kv_heads (at most 128 times), sq <= sk; addresses and strides in whole 16 bytes.
 cudaError_t launch_prompt_attention(const PromptParams& p, DType dt, cudaStream_t stream);
 

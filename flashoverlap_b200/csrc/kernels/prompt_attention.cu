@@ -133,6 +133,12 @@ struct PromptArgs {
   PromptParams p;
   CUtensorMap q, k, v;
   int group, tokens;         // query heads of a head, tokens of a tile
+  // Few pairs of tiles: the keys of a pair are divided over `parts` CTAs, which leave unscaled results in fp32, for each row
+  // the largest score (times log2 e) and the sum of weights, and for each tile whether a value was not finite.
+  int parts;
+  float* part_out;
+  float2* part_ml;
+  int* part_odd;
   int blocks, q_batch, k_batch, v_batch, k_head, v_head, q_head;  // pairs of tiles; 0 where a dimension is broadcast, else 1
   float scale_log2;
 };
@@ -222,11 +228,18 @@ __device__ __forceinline__ void hide(uint32_t (&s)[32], uint32_t see) {
 struct PromptPair {
   int b, kv_head, t0, length;  // t0: first token of the first tile
   SeenTiles tiles;
-  int n;  // tiles of keys; 0: no row sees anything
+  int n;      // tiles of keys that this CTA takes; 0: none
+  int first;  // the first of them
+  __device__ __forceinline__ int key(int j) const { return tiles.start(first + j); }
 };
 __device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index) {
   const PromptParams& p = a.p;
   PromptPair r;
+  int part = 0;
+  if (a.parts > 1) {
+    part = index % a.parts;
+    index /= a.parts;
+  }
   // late tokens first: they see the most keys
   const int per = p.batch * p.kv_heads;
   const int qb = index / per, rest = index - qb * per;
@@ -236,7 +249,13 @@ __device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index
   r.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + r.b), 0), p.sk);
   const int p0 = p.sk - p.sq + r.t0, p1 = p.sk - p.sq + min(r.t0 + 2 * a.tokens, p.sq) - 1;
   r.tiles = seen_tiles(p0, p1, r.length, p.window, p.sinks, kTileKeys, 1);
-  r.n = p0 < r.length ? r.tiles.count() : 0;
+  r.n = p0 < r.length ? r.tiles.count() : 0;  // 0: no row sees anything
+  r.first = 0;
+  if (a.parts > 1) {
+    const int per = (r.n + a.parts - 1) / a.parts;
+    r.first = min(part * per, r.n);
+    r.n = min(per, r.n - r.first);
+  }
   return r;
 }
 // Whether every row of tile i (0, 1) sees all of a tile of keys.
@@ -287,6 +306,94 @@ __device__ __forceinline__ int claimed_cta(const void* answer) {
       : "r"(ptx::smem_u32(answer))
       : "memory");
   return ok ? static_cast<int>(x) : -1;
+}
+
+// A part's results of one row: 32 columns at a time through the warp's stage, so that whole lines are stored.
+template <int D>
+__device__ __forceinline__ void store_part(const PromptArgs& a, int index, int tile, int row, uint32_t stage, uint32_t t_o,
+                                           bool any, bool odd, float m, float l) {
+  const int lane = row & 31;
+  const long long first = (static_cast<long long>(index) * 2 + tile) * kTileRows;
+  a.part_ml[first + row] = any && m != kLowest ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
+  if (row == 0) a.part_odd[index * 2 + tile] = odd;
+  if (!any) return;
+#pragma unroll
+  for (int q = 0; q < D / 32; ++q) {
+    uint32_t o[32];
+    ptx::tmem_ld_32x32b_x32(t_o + q * 32, o);
+    ptx::tmem_ld_wait_for(o);
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      ptx::st_shared_v4(stage + lane * 128 + ((e ^ (lane & 7)) << 4), make_uint4(o[e * 4], o[e * 4 + 1], o[e * 4 + 2], o[e * 4 + 3]));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int from = e * 4 + (lane >> 3), chunk = lane & 7;
+      const uint4 v = ptx::ld_shared_v4(stage + from * 128 + ((chunk ^ (from & 7)) << 4));
+      ptx::st_v4(a.part_out + (first + (row & ~31) + from) * D + q * 32 + chunk * 4, v);
+    }
+  }
+}
+
+// Joins the parts of a pair's rows, a warp for each row; lanes take columns.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
+  constexpr int V = D / 32, kBatch = 4;
+  ptx::wait_for_previous_kernel();
+  ptx::allow_next_kernel();
+  const PromptParams& p = a.p;
+  const int lane = threadIdx.x & 31, pair = blockIdx.x;
+  const int rows = a.group * a.tokens;
+  const int x = blockIdx.y * 8 + (threadIdx.x >> 5);  // rows of both tiles
+  if (x >= 2 * rows) return;
+  const int tile = x / rows, row = x - tile * rows;
+  const PromptPair r = prompt_pair(a, pair * a.parts);
+  const int t = r.t0 + tile * a.tokens + row / a.group, head = r.kv_head * a.group + row % a.group;
+  if (t >= p.sq) return;
+  bool odd = false;
+  float acc[V] = {}, sum = 0.f, most = -INFINITY;
+  for (int i0 = 0; i0 < a.parts; i0 += kBatch) {
+    float2 ml[kBatch];
+    float y[kBatch][V];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int part = pair * a.parts + min(i0 + k, a.parts - 1);
+      const long long at = (static_cast<long long>(part) * 2 + tile) * kTileRows + row;
+      ml[k] = a.part_ml[at];
+      odd |= a.part_odd[part * 2 + tile] != 0;
+      // (a part that saw nothing has written no results)
+      const bool any = i0 + k < a.parts && (ml[k].x != -INFINITY || ml[k].y != 0.f);
+      if (!any) ml[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int v = 0; v < V; ++v) y[k][v] = any ? a.part_out[at * D + lane * V + v] : 0.f;
+    }
+    float top = most;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) top = fmaxf(top, ml[k].x);
+    const float base = top == -INFINITY ? 0.f : top;
+    const float old = exp2_fast(most - base);
+    most = top;
+    sum *= old;
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] *= old;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w = exp2_fast(ml[k].x - base);
+      sum += ml[k].y * w;
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] += y[k][v] * w;
+    }
+  }
+  if (odd) {
+    exact_row<D, BF16>(p, r.b, t, head, r.length, a.scale_log2);
+    return;
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<long long>(r.b) * p.sq + t) * p.heads + head) * D + lane * V;
+#pragma unroll
+  for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t*>(dst + v) = inv == 0.f ? 0u : pack<BF16>(acc[v] * inv, acc[v + 1] * inv);
 }
 
 constexpr int kChecks = 8;    // tiles of values that may have been looked at and not used: more than the ring holds
@@ -404,7 +511,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           }
         }
         for (int j = 0; ok && j < r.n; ++j) {
-          const int key = r.tiles.start(j);
+          const int key = r.key(j);
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
             if (buf.round > 0) ok = ok && wait(&kv_empty[buf.at], (buf.round - 1) & 1u);
@@ -542,7 +649,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     for (int it = 0; ok && index >= 0; ++it) {
       const PromptPair r = prompt_pair(a, index);
       for (int j = 0; ok && j < r.n; ++j, ++tiles) {
-        const int first_key = r.tiles.start(j);
+        const int first_key = r.key(j);
         buf.next();
         ok = wait_warp(&kv_full[buf.at], buf.round & 1u);
         if (!ok) break;
@@ -593,7 +700,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
       float m = kLowest, l = 0.f;
       for (int j = 0; j < r.n; ++j, ++tiles) {
-        const int first_key = r.tiles.start(j);
+        const int first_key = r.key(j);
         const bool masked = !sees_whole(a, r, tile, first_key);
         ok = wait_warp(&s_full[tile], tiles & 1u);
         if (!ok) break;
@@ -695,7 +802,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         if (lane == 0) atomicMin(&unfinished, it);
         break;
       }
-      if (!by_rows) {
+      if (a.parts > 1) {
+        store_part<D>(a, index, tile, row, stage + warp * kStageBytes, t_o, r.n > 0, by_rows, m, l);
+        ptx::tc_fence_before_sync();
+      } else if (!by_rows) {
         // Through shared memory, so that a store instruction writes four whole lines and not parts of 32: a row's chunks of 16
         // bytes go in where the row's number puts them, eight lanes read a row.
         const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -766,6 +876,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       else if (pending >= 0 && ptx::mbar_try_wait(&next_full[pending & 1], (pending >> 1) & 1u)) index = claimed_cta(&answers[pending & 1]);
       if (index < 0) continue;
       const PromptPair r = prompt_pair(a, index);
+      if (a.parts > 1) {
+        for (int x = threadIdx.x; x < 2 * kTileRows; x += kPromptThreads) {
+          a.part_ml[static_cast<long long>(index) * 2 * kTileRows + x] = make_float2(0.f, NAN);
+          if (x < 2) a.part_odd[index * 2 + x] = 0;
+        }
+        continue;
+      }
       for (int x = threadIdx.x; x < rows * (D / 8); x += kPromptThreads) {
         const int y = x / (D / 8), t = r.t0 + y / a.group;
         if (t < p.sq) {
@@ -819,6 +936,30 @@ bool fits_tiles(const PromptParams& p) {
          (group == 1 || p.q_stride[2] != 0);
 }
 
+// How a call is divided: pairs of tiles, and over how many CTAs the keys of a pair.  Up to half of the SMs' number of pairs
+// leave SMs without work; each part has at least kPartTiles tiles, since what a CTA costs however little it does, and
+// the second kernel, take as long as some of them.
+constexpr int kPartTiles = 3;
+struct PromptGrid {
+  int tokens, blocks, parts;
+  long long pairs;
+};
+PromptGrid prompt_grid(const PromptParams& p) {
+  PromptGrid g;
+  g.tokens = kTileRows / (p.heads / p.kv_heads);
+  g.blocks = (p.sq + 2 * g.tokens - 1) / (2 * g.tokens);
+  g.pairs = static_cast<long long>(g.blocks) * p.batch * p.kv_heads;
+  g.parts = 1;
+  const int sms = device_sm_count();
+  if (g.pairs * 2 <= sms) {
+    const int t0 = (g.blocks - 1) * 2 * g.tokens;
+    const int tiles = seen_tiles(p.sk - p.sq + t0, p.sk - 1, p.sk, p.window, p.sinks, kTileKeys, 1).count();
+    const int parts = std::min(sms / static_cast<int>(g.pairs), tiles / kPartTiles);
+    if (parts > 1) g.parts = parts;
+  }
+  return g;
+}
+
 template <int D, bool BF16>
 cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   if (!fits_tiles(p)) {
@@ -830,8 +971,10 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   std::memset(&a, 0, sizeof(a));
   a.p = p;
   a.group = p.heads / p.kv_heads;
-  a.tokens = kTileRows / a.group;
-  a.blocks = (p.sq + 2 * a.tokens - 1) / (2 * a.tokens);
+  const PromptGrid g = prompt_grid(p);
+  a.tokens = g.tokens;
+  a.blocks = g.blocks;
+  a.parts = g.parts;
   a.scale_log2 = p.scale * kLog2e;
   a.q_batch = p.q_stride[0] != 0;
   a.q_head = p.q_stride[2] != 0;
@@ -845,15 +988,34 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
       !make_map(&a.v, p.v, dt, D, {p.sk, p.kv_heads, p.batch}, {p.v_stride[1], p.v_stride[2], p.v_stride[0]}, {kTileKeys, 1})) {
     return cudaErrorInvalidValue;
   }
-  const long long grid = static_cast<long long>(a.blocks) * p.batch * p.kv_heads;
+  const long long grid = g.pairs * g.parts;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
+  if (a.parts > 1) {
+    char* ws = static_cast<char*>(p.workspace);
+    a.part_out = reinterpret_cast<float*>(ws);
+    ws += sizeof(float) * 2 * kTileRows * D * grid;
+    a.part_ml = reinterpret_cast<float2*>(ws);
+    ws += sizeof(float2) * 2 * kTileRows * grid;
+    a.part_odd = reinterpret_cast<int*>(ws);
+  }
   cudaError_t e = allow_smem(prompt_attention_kernel<D, BF16>, prompt_smem_bytes<D>());
   if (e != cudaSuccess) return e;
-  return launch_after(prompt_attention_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), kPromptThreads,
-                      prompt_smem_bytes<D>(), stream, 1, a);
+  e = launch_after(prompt_attention_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), kPromptThreads, prompt_smem_bytes<D>(),
+                   stream, 1, a);
+  if (e != cudaSuccess || a.parts == 1) return e;
+  const int rows = 2 * a.tokens * a.group;
+  return launch_after(prompt_join_kernel<D, BF16>, dim3(static_cast<unsigned>(g.pairs), (rows + 7) / 8), 256, 0, stream, 1, a);
 }
 
 }  // namespace
+
+size_t prompt_workspace_bytes(const PromptParams& p) {
+  if (p.batch == 0 || p.sq == 0 || !fits_tiles(p)) return 0;
+  const PromptGrid g = prompt_grid(p);
+  if (g.parts == 1) return 0;
+  const size_t tiles = static_cast<size_t>(g.pairs) * g.parts * 2;
+  return tiles * kTileRows * (p.head_dim * sizeof(float) + sizeof(float2)) + tiles * sizeof(int);
+}
 
 cudaError_t launch_prompt_attention(const PromptParams& p, DType dt, cudaStream_t stream) {
   if (p.batch == 0 || p.sq == 0) return cudaSuccess;
