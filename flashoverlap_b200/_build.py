@@ -32,6 +32,7 @@ SOURCES = [
     "kernels/prompt_attention.cu",
     "runtime/symm_heap.cpp",
     "runtime/engine.cpp",
+    "runtime/page_pool.cpp",
     "api/nccl_utils.cpp",
     "api/overlap_impl.cpp",
     "api/baseline_impl.cpp",

@@ -18,6 +18,8 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.attention import prompt_attention
+
 
 def _rms(x, w, eps):
     xf = x.float()
@@ -26,7 +28,8 @@ def _rms(x, w, eps):
 
 class TPDecoderBlock(nn.Module):
     def __init__(self, impl, hidden: int = 8192, ffn: int = 28672, n_heads: int = 64, n_kv_heads: int = 8,
-                 eps: float = 1e-5, algo: int = 8, dtype=torch.bfloat16, device=None, seed: int = 0):
+                 eps: float = 1e-5, algo: int = 8, dtype=torch.bfloat16, device=None, seed: int = 0,
+                 window: int = 0, sinks: int = 0):
         super().__init__()
         self.impl = impl
         self.world = dist.get_world_size() if dist.is_initialized() else 1
@@ -37,6 +40,7 @@ class TPDecoderBlock(nn.Module):
         self.head_dim = hidden // n_heads
         self.heads = n_heads // ws
         self.kv_heads = max(1, n_kv_heads // ws)
+        self.window, self.sinks = window, sinks
         dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
         g = torch.Generator(device="cpu").manual_seed(seed * 1000 + self.rank)
 
@@ -55,8 +59,15 @@ class TPDecoderBlock(nn.Module):
         self.norm_next = nn.Parameter((1 + 0.1 * torch.randn(hidden, generator=gn)).to(dev, dtype), requires_grad=False)
 
     # ---- shared pieces ----------------------------------------------------
+    def _heads(self, qkv, *shape):
+        """Queries, keys and values as views [*shape, heads, head_dim] of the projection's rows."""
+        parts = qkv.split([n * self.head_dim for n in (self.heads, self.kv_heads, self.kv_heads)], dim=-1)
+        return [x.unflatten(-1, (-1, self.head_dim)).unflatten(0, shape) for x in parts]
+
     def _attention(self, qkv, batch, seq):
         hd, h, kv = self.head_dim, self.heads, self.kv_heads
+        if self.window:
+            return prompt_attention(*self._heads(qkv, batch, seq), window=self.window, sinks=self.sinks).view(-1, h * hd)
         q, k, v = qkv.split([h * hd, kv * hd, kv * hd], dim=-1)
         q = q.reshape(batch, seq, h, hd).transpose(1, 2)
         k = k.reshape(batch, seq, kv, hd).transpose(1, 2)
@@ -76,15 +87,45 @@ class TPDecoderBlock(nn.Module):
 
     # ---- fused path ---------------------------------------------------------
     @torch.no_grad()
-    def forward(self, h_norm, resid, batch, seq):
+    def forward(self, h_norm, resid, batch, seq, cache=None, seqs=None):
         """h_norm: normalised block input [tokens, hidden] (replicated), resid: the
         residual stream [tokens, hidden].  Returns (next layer's QKV for all
-        tokens [tokens, qkv_rows], new residual shard [tokens/world, hidden])."""
-        impl, a = self.impl, self.algo
-        T = h_norm.shape[0]
-        qkv = torch.empty((T, self.w_qkv.shape[0]), dtype=h_norm.dtype, device=h_norm.device)
-        impl.cutlass_gemm(h_norm, self.w_qkv, qkv, self._fit(T, self.w_qkv.shape[0]))
-        attn = self._attention(qkv, batch, seq)
+        tokens [tokens, qkv_rows], new residual shard [tokens/world, hidden]).
+        With a ``cache`` (PagedKVCache) the tokens' keys and values are stored as the first
+        of its sequences ``seqs``, which have none yet."""
+        qkv = self._project(h_norm)
+        if cache is not None:
+            if any(cache.length(s) for s in seqs):
+                raise ValueError("forward stores whole prompts: the sequences must be empty")
+            _, k, v = self._heads(qkv, batch, seq)
+            cache.append(seqs, k, v)
+        return self._after(self._attention(qkv, batch, seq), resid)
+
+    @torch.no_grad()
+    def decode(self, h_norm, resid, cache, seqs):
+        """One new token of each of the cache's sequences ``seqs``: h_norm and resid are [len(seqs), hidden].
+        The token's key and value are stored, and it attends over all of its sequence.  Returns (next layer's QKV
+        [len(seqs), qkv_rows], new residual: this rank's share of the rows, which are padded to 128 a rank)."""
+        n = len(seqs)
+        pad = -n % (128 * self.world)
+        h_norm, resid = (F.pad(x, (0, 0, 0, pad)) if pad else x for x in (h_norm, resid))
+        qkv = self._project(h_norm)
+        q, k, v = self._heads(qkv[:n], n, 1)
+        cache.append(seqs, k, v)
+        attn = qkv.new_zeros((n + pad, self.heads * self.head_dim))
+        cache.attend(seqs, q[:, 0], window=self.window, sinks=self.sinks, out=attn[:n].view(n, self.heads, self.head_dim))
+        qkv_next, h3 = self._after(attn, resid)
+        return qkv_next[:n], h3
+
+    def _project(self, h_norm):
+        qkv = torch.empty((h_norm.shape[0], self.w_qkv.shape[0]), dtype=h_norm.dtype, device=h_norm.device)
+        self.impl.cutlass_gemm(h_norm, self.w_qkv, qkv, self._fit(*qkv.shape))
+        return qkv
+
+    def _after(self, attn, resid):
+        """What follows the attention."""
+        impl, T = self.impl, attn.shape[0]
+        a = self._own_tile(T)
         o = impl.gemm_allreduce_fused(attn, self.w_o, None, self.eps, a)          # GEMM + all-reduce
         h2, m_in = self._add_norm(resid, o, self.norm_attn)
         act = self._gated(m_in)
@@ -120,6 +161,13 @@ class TPDecoderBlock(nn.Module):
         gu = torch.empty((T, rows), dtype=x.dtype, device=x.device)
         self.impl.cutlass_gemm(x, self.w_gate_up, gu, algo)
         return self._mlp_act(gu)
+
+    def _own_tile(self, T):
+        """The block's tile configuration; for few tokens (decode pads them to 128 a rank) one that divides them."""
+        from ..utils.config import ALGO_TILES
+
+        share = T // self.world
+        return self._fit(share, self.hidden) if share % 128 == 0 and share % ALGO_TILES[self.algo][0] else self.algo
 
     def _fit(self, M, N):
         """The preferred tile configuration if it divides the shape, else a smaller one."""

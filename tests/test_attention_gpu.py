@@ -479,3 +479,99 @@ def test_tensors_on_another_device_than_the_current_one():
     dev = torch.device("cuda", 1)
     got = ops.paged_attention(q.to(dev), p.cache.to(dev), p.table.to(dev), p.lengths.to(dev))
     assert torch.equal(got.cpu(), want.cpu())
+
+
+# ---- a cache with its pool, and the decoder block on it ---------------------------
+def test_cache_of_sequences_that_fork_and_move():
+    from flashoverlap_b200.models import PagedKVCache
+
+    kv, dim, heads, page = 2, 64, 6, 16
+    cache = PagedKVCache(60, page, kv, dim, dtype=BF16)
+    tokens = {}
+
+    def put(seqs, n, seed, counts=None):
+        k, v = (randn(len(seqs), n, kv, dim, dtype=BF16, seed=seed + i) for i in (0, 1))
+        cache.append(seqs, k, v, counts)
+        for i, s in enumerate(seqs):
+            m = n if counts is None else counts[i]
+            old = tokens.get(s, (k[0, :0], v[0, :0]))
+            tokens[s] = (torch.cat([old[0], k[i, :m]]), torch.cat([old[1], v[i, :m]]))
+
+    def look(window=0, sinks=0):
+        seqs = sorted(tokens)
+        q = randn(len(seqs), heads, dim, dtype=BF16, seed=len(seqs))
+        got = cache.attend(seqs, q, window=window, sinks=sinks)
+        for i, s in enumerate(seqs):
+            n = len(tokens[s][0])
+            assert cache.length(s) == n
+            for h in range(heads):
+                want, tol = attend(q[i, h][None], tokens[s][0][:, h // 3], tokens[s][1][:, h // 3], n - 1, n, window, sinks)
+                check(got[i, h][None], want, tol, f"sequence {s}")
+
+    a, b, c = (cache.add() for _ in range(3))
+    put([a, b, c], 50, 1, counts=[50, 32, 7])
+    look()
+    d, e = cache.fork(a), cache.fork(b)      # 50 tokens: a page is copied; 32: none is
+    tokens[d], tokens[e] = tokens[a], tokens[b]
+    put([a, d, e, b], 1, 10)                 # each goes on by itself
+    put([d], 40, 20)
+    look()
+    cache.free(a)
+    del tokens[a]
+    look(window=20, sinks=3)
+    assert cache.compact() > 0 and cache.compact() == 0
+    look()
+    put([c, e], 100, 30, counts=[100, 0])
+    look()
+    # what is refused leaves everything as it was
+    free = cache.pool.free_pages()
+    x = randn(1, 2000, kv, dim, dtype=BF16)
+    for call in (lambda: cache.append([c], x, x), lambda: cache.append([c, c], x[:, :2].expand(2, -1, -1, -1), x[:, :2].expand(2, -1, -1, -1)),
+                 lambda: cache.append([c], x[:, :2], x[:, :3]), lambda: cache.append([c], x[:, :2].half(), x[:, :2].half()),
+                 lambda: cache.append([c], x[:, :2], x[:, :2], [3]), lambda: cache.append([99], x[:, :2], x[:, :2]),
+                 lambda: cache.append([c], x[:, :2].cpu(), x[:, :2].cpu())):
+        with pytest.raises((RuntimeError, ValueError)):
+            call()
+    assert cache.pool.free_pages() == free
+    look()
+    y = randn(1, 3, kv, dim + 3, dtype=BF16)[..., 3:]      # rows off 16-byte boundaries are copied first
+    cache.append([c], y, y)
+    tokens[c] = tuple(torch.cat([t, y[0]]) for t in tokens[c])
+    look()
+
+
+@pytest.mark.parametrize("hidden,heads,kv_heads,window,sinks", [(512, 8, 2, 0, 0), (1024, 8, 8, 50, 3), (512, 4, 1, 0, 0)])
+def test_decoder_block_token_by_token(hidden, heads, kv_heads, window, sinks):
+    # prompts of 128 tokens, then single tokens: as a prompt of all of them
+    from flashoverlap_b200.models import PagedKVCache
+    from flashoverlap_b200.models.decoder_block import TPDecoderBlock
+
+    impl = torch.classes.flashoverlap_class.OverlapImpl()
+    impl.nccl_init(0, 1, [0] * 16)
+    impl.cutlass_init()
+    impl.overlap_init()
+    block = TPDecoderBlock(impl, hidden, 512, heads, kv_heads, 1e-5, 3, dtype=BF16, window=window, sinks=sinks)
+    batch, first, total = 2, 128, 192
+    resid = randn(batch, total, hidden, dtype=BF16, seed=5)
+    h = (resid.float() * torch.rsqrt(resid.float().pow(2).mean(-1, keepdim=True) + 1e-5)).to(BF16)
+    want_q, want_r = (x.view(batch, total, -1) for x in block.forward_reference(h.view(-1, hidden), resid.view(-1, hidden), batch, total))
+    cache = PagedKVCache(40, 16, kv_heads, hidden // heads, dtype=BF16)
+    seqs = [cache.add() for _ in range(batch)]
+    q, r = block(h[:, :first].reshape(-1, hidden), resid[:, :first].reshape(-1, hidden), batch, first, cache=cache, seqs=seqs)
+
+    def close(got, want):
+        # five products of 16-bit values in a row, each rounded: 2^-8 of the largest value and as much for what follows from it
+        assert (got.float() - want.float()).abs().max() <= 2 ** -5 * want.float().abs().max()
+
+    close(q.view(batch, first, -1), want_q[:, :first])
+    close(r.view(batch, first, -1), want_r[:, :first])
+    for t in range(first, first + 20):
+        q, r = block.decode(h[:, t], resid[:, t], cache, seqs)
+        assert q.shape[0] == batch
+        close(q, want_q[:, t])
+        close(r[:batch], want_r[:, t])
+    assert [cache.length(s) for s in seqs] == [first + 20] * batch
+    with pytest.raises(ValueError, match="empty"):
+        block(h[:, :first].reshape(-1, hidden), resid[:, :first].reshape(-1, hidden), batch, first, cache=cache, seqs=seqs)
+    torch.cuda.synchronize()
+    impl.check_status()
