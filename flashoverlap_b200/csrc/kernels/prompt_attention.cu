@@ -766,27 +766,38 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
         const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
         Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
+        // Eight pairs at a time: their arguments, their powers, then what is done with them, so that nothing waits for the
+        // power just asked for.
+        uint32_t w[2][32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[32];
+        for (int g = 0; g < 8; ++g) {
+          Pair x[8];
+          float2 y[8];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const uint32_t* src = s[half * 2 + (e >> 4)] + (e & 15) * 2;
-            const Pair x = fma2(make_pair(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, base2);
-            float2 y;
-            if (e % kPolyEvery == kPolyEvery - 1) {
-              y = exp2_poly(x);
-            } else {
-              y = split(x);
-              y = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-            }
-            sum[e & 1] = add2(sum[e & 1], make_pair(y.x, y.y));
-            w[e] = pack<BF16>(y.x, y.y);
+          for (int e = 0; e < 8; ++e) {
+            const uint32_t* src = s[g >> 1] + (g & 1) * 16 + e * 2;
+            x[e] = fma2(make_pair(__uint_as_float(src[0]), __uint_as_float(src[1])), c2, base2);
           }
-          tmem_st_32x32b_x32(t_p + half * 32, w);
-          tmem_st_wait();
-          ptx::tc_fence_before_sync();
-          ptx::mbar_arrive(&p_full[tile][half]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            if (e % kPolyEvery == kPolyEvery - 1) {
+              y[e] = exp2_poly(x[e]);
+            } else {
+              y[e] = split(x[e]);
+              y[e] = make_float2(exp2_fast(y[e].x), exp2_fast(y[e].y));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            sum[e & 1] = add2(sum[e & 1], make_pair(y[e].x, y[e].y));
+            w[g >> 2][(g & 3) * 8 + e] = pack<BF16>(y[e].x, y[e].y);
+          }
+          if (g == 3 || g == 7) tmem_st_32x32b_x32(t_p + (g >> 2) * 32, w[g >> 2]);
+          if (g == 3 || g == 7) {  // (the first half's way to TMEM is under the next weights)
+            tmem_st_wait();
+            ptx::tc_fence_before_sync();
+            ptx::mbar_arrive(&p_full[tile][g == 7]);
+          }
         }
         const float2 total = split(add2(sum[0], sum[1]));
         l += total.x + total.y;
