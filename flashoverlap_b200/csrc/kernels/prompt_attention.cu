@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
-constexpr uint64_t kDeadlineNs = 4000000000ull;  // of a wait; nothing here takes a thousandth of it
+constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
 constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
@@ -456,11 +456,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const uint32_t tmem = tmem_slot;
   ptx::wait_for_previous_kernel();
 
-  const uint64_t deadline = ptx::globaltimer_ns() + kDeadlineNs;
+  // Each wait has a limit of its own: a CTA may work for long.  Once one has run out, all give up.
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ptx::mbar_wait(bar, parity, deadline)) return true;
-    *const_cast<volatile int*>(&failed) = 1;
-    return false;
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    uint64_t deadline = 0;
+    for (uint32_t tries = 1;; ++tries) {
+      if (ptx::mbar_try_wait(bar, parity)) return true;
+      if ((tries & 0x3ffu) == 0u) {
+        const uint64_t now = ptx::globaltimer_ns();
+        if (deadline == 0) deadline = now + kDeadlineNs;
+        if (now > deadline || *const_cast<volatile int*>(&failed) != 0) {
+          *const_cast<volatile int*>(&failed) = 1;
+          return false;
+        }
+      }
+    }
   };
   // the lanes of a warp go on, or give up, together
   auto wait_warp = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };

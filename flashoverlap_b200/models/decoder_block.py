@@ -106,6 +106,8 @@ class TPDecoderBlock(nn.Module):
         """One new token of each of the cache's sequences ``seqs``: h_norm and resid are [len(seqs), hidden].
         The token's key and value are stored, and it attends over all of its sequence.  Returns (next layer's QKV
         [len(seqs), qkv_rows], new residual: this rank's share of the rows, which are padded to 128 a rank)."""
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"attention over a cache takes heads of 64 or 128 values, not {self.head_dim}")
         n = len(seqs)
         pad = -n % (128 * self.world)
         h_norm, resid = (F.pad(x, (0, 0, 0, pad)) if pad else x for x in (h_norm, resid))

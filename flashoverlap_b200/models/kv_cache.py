@@ -25,6 +25,8 @@ class PagedKVCache:
         if kv_heads < 1 or page_size < 1 or head_dim < 1 or head_dim % 8:
             raise ValueError("kv_heads, page_size and head_dim must be positive, head_dim a multiple of 8")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+        if device.type != "cuda":
+            raise ValueError("the cache lives on a GPU")
         self.data = torch.zeros((pages, 2, kv_heads, page_size, head_dim), dtype=dtype, device=device)
         self.pool = torch.classes.flashoverlap_class.PagePool(pages, page_size)
 

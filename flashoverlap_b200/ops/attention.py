@@ -27,7 +27,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
 
     The queries are the last ``sq`` of the ``sk`` tokens.  ``lengths[batch]`` (int32): how many of the ``sk`` tokens
     sequence b has; rows behind them are zero, and what stands there is not read into any result.  Strided views are fine
-    as long as rows are contiguous and begin on 16-byte boundaries.  ``scale`` defaults to ``head_dim ** -0.5``."""
+    as long as rows are contiguous and begin on 16-byte boundaries.  ``scale`` defaults to ``head_dim ** -0.5``.  ``out`` must
+    be contiguous and may not lie between the first and the last value of q, k or v."""
     _check(q)
     if out is None:
         return torch.ops.flashoverlap_op.prompt_attention_new.default(q, k, v, window, sinks, lengths, scale)

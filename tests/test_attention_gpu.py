@@ -575,3 +575,107 @@ def test_decoder_block_token_by_token(hidden, heads, kv_heads, window, sinks):
         block(h[:, :first].reshape(-1, hidden), resid[:, :first].reshape(-1, hidden), batch, first, cache=cache, seqs=seqs)
     torch.cuda.synchronize()
     impl.check_status()
+
+
+# ---- forms that the sizes above do not take -----------------------------------------
+@pytest.mark.parametrize("dtype", [FP16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv,page,window,sinks", [(16, 1, 24, 0, 0), (40, 1, 64, 0, 0), (10, 2, 16, 3500, 17), (8, 1, 128, 0, 0)])
+def test_single_tokens_of_long_sequences(dtype, dim, heads, kv, page, window, sinks):
+    # more tiles than a cluster takes: stretches that begin and end anywhere, joined by the second kernel
+    lengths = [5000, 0, 4999, 1, 777, 4097]
+    p = Paged(lengths, kv, dim, page, dtype, seed=heads)
+    q = randn(len(lengths), heads, dim, dtype=dtype, seed=9)
+    got = ops.paged_attention(q, p.cache, p.table, p.lengths, window=window, sinks=sinks)
+    p.check(q, got, window, sinks)
+    assert torch.equal(got, ops.paged_attention(q, p.cache, p.table, p.lengths, window=window, sinks=sinks))
+    table = p.table.clone()
+    table[2, 3] = -1                     # visible, or hidden by the window
+    got = ops.paged_attention(q, p.cache, table, p.lengths, window=window, sinks=sinks)
+    p.check(q, got, window, sinks, only=(0, 1, 3, 4, 5) + ((2,) if window else ()))
+    assert window or got[2].isnan().all()
+
+
+@pytest.mark.parametrize("scale", [-0.07, 0.0, 3.0])
+def test_scales_of_single_tokens(scale):
+    for lengths, dim in (([40, 300, 5], 128), ([9000, 33], 64)):
+        p = Paged(lengths, 1, dim, 16, BF16)
+        q = randn(len(lengths), 5, dim, dtype=BF16)
+        p.check(q, ops.paged_attention(q, p.cache, p.table, p.lengths, scale=scale), scale=scale)
+
+
+def test_sequences_in_the_hundreds():
+    # more sequences than a warp looks at together, most of them short or empty; the table is wider than any needs
+    lengths = [(i * 37) % 61 if i % 3 else 0 for i in range(333)] + [2900]
+    p = Paged(lengths, 2, 64, 16, FP16, width=200)
+    q = randn(len(lengths), 6, 64, dtype=FP16)
+    got = ops.paged_attention(q, p.cache, p.table, p.lengths)
+    p.check(q, got, only=list(range(0, 334, 7)) + [333, 332, 331])
+    assert not got[::3][:111].any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("batch,sq,sk,heads,kv,window,sinks", [(3, 1500, 1500, 16, 4, 300, 5), (40, 300, 300, 8, 8, 0, 0),
+                                                               (2, 30, 2000, 8, 1, 0, 0), (1, 100, 1700, 6, 2, 900, 130)])
+def test_many_and_few_pairs_with_values_that_are_not_finite(dim, batch, sq, sk, heads, kv, window, sinks):
+    # more pairs of tiles than SMs, and so few that their keys are divided; lengths that leave pairs without keys
+    q = randn(batch, sq, heads, dim, dtype=BF16, seed=1)
+    k, v = randn(batch, sk, kv, dim, dtype=BF16, seed=2), randn(batch, sk, kv, dim, dtype=BF16, seed=3)
+    lengths = [(sk * (b + 1)) // batch - 3 * b for b in range(batch)]
+    lengths[-1] = sk
+    clean = v.clone()
+    for b, n in enumerate(lengths):
+        v[b, n:], k[b, n:] = float("inf"), float("nan")
+    bad = sk - sq // 2
+    v[0, bad, :, 5] = float("nan")
+    v[-1, bad, 0, 3] = float("-inf")
+    got = ops.prompt_attention(q, k, v, window=window, sinks=sinks, lengths=ints(*lengths))
+    group = heads // kv
+    pos = torch.arange(sk - sq, sk)
+    for b in {0, batch // 2, batch - 1}:
+        for h in {0, heads - 1}:
+            want, tol = attend(q[b, :, h], k[b, :, h // group], clean[b, :, h // group], sk - sq, lengths[b], window, sinks)
+            hit = (pos >= bad) & (pos < lengths[b]) & (bad < lengths[b])
+            if window:
+                hit &= pos < bad + window
+            if b not in (0, batch - 1) or (b == batch - 1 and b != 0 and h // group != 0):
+                hit &= False
+            check(got[b, ~hit, h], want[~hit], tol[~hit], f"sequence {b}, head {h}")
+            col = 5 if b == 0 else 3
+            if hit.any():
+                assert not got[b, hit, h, col].isfinite().any()
+
+
+def test_prompts_on_two_streams():
+    sets = [[randn(1, n, h, 128, dtype=FP16, seed=n + h) for h in (8, 2, 2)] for n in (1900, 1901)]
+    want = [ops.prompt_attention(*x, window=500, sinks=2) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for x, s in zip(sets, streams):
+            with torch.cuda.stream(s):
+                got.append(ops.prompt_attention(*x, window=500, sinks=2))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_a_split_prompt_in_two_graphs():
+    # each graph has partial results of its own
+    sets = [[randn(1, n, h, 64, dtype=BF16, seed=n + h) for n, h in ((20, 8), (3000, 1), (3000, 1))] for _ in range(2)]
+    sets[1] = [x + 1 for x in sets[1]]
+    want = [ops.prompt_attention(*x) for x in sets]
+    graphs, outs = [], []
+    for x in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.prompt_attention(*x))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for o, w in zip(outs, want))
