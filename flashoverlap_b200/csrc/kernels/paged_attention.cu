@@ -14,9 +14,9 @@
 // stretch.
 //
 // Measured, call after call over three sets of inputs, caches larger than L2: 64 sequences of 1 to 4999 tokens, 32 heads on 8
-// of 128, pages of 64: 114 us (5.75 TB/s); two of 100003 and 131072 tokens, 8 heads on 1: 28 us (4.2 TB/s; 1.5 us until a CTA
+// of 128, pages of 64: 109 us (6.0 TB/s); two of 100003 and 131072 tokens, 8 heads on 1: 27 us (4.4 TB/s; 1.4 us until a CTA
 // knows its stretch, 19 at 6.2 TB/s, then the join: 1 us until its kernel runs, 3 for 150 parts of a head); 48 of up to 30000
-// tokens seen through a window of 4096, heads of 64, pages of 24 tokens: 28 us (3.3 TB/s).  One sequence of 900 tokens: 6 us
+// tokens seen through a window of 4096, heads of 64, pages of 24 tokens: 24.5 us (3.8 TB/s).  One sequence of 900 tokens: 6 us
 // on the device, 7.4 a call.  With query heads as rows (16, of which 8 are filled) and addresses worked out for every row,
 // a strip took 840 instructions of a warp and the first of these cases 129 us, also when everything came from L2.
 #include <algorithm>
@@ -161,10 +161,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     ic.i = rank * per;
     ic.left = max(min(per, ic.q.count - ic.i), 0);
   } else {
-    int total = 0, mine = 0;
+    int total = 0, mine = 0, n[kAhead];
 #pragma unroll 1
     for (int s0 = 0; s0 < p.seqs; s0 += 32 * kAhead) {  // (kAhead lengths of a lane are asked for together)
-      int n[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
         const int s = s0 + k * 32 + lane;
@@ -188,7 +187,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
     int before = 0;
 #pragma unroll 1
     for (int s0 = 0;; s0 += 32) {
-      if (p.seqs > 32) mine = s0 + lane < p.seqs ? sequence(p, __ldg(p.lengths + s0 + lane), TILE).count : 0;
+      if (p.seqs > 32) {
+        n[0] = s0 + lane < p.seqs ? __ldg(p.lengths + s0 + lane) : 0;
+        mine = s0 + lane < p.seqs ? sequence(p, n[0], TILE).count : 0;
+      }
       // most chunks end before the stretch begins
       const int all = __reduce_add_sync(0xffffffffu, mine);
       if ((before + all) * heads <= at_tile) {
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
       // the first sequence that ends behind the stretch's beginning
       const int which = __ffs(__ballot_sync(0xffffffffu, (before + sum) * heads > at_tile)) - 1;
       ic.s = s0 + which;
-      ic.q = sequence(p, __ldg(p.lengths + ic.s), TILE);
+      ic.q = sequence(p, __shfl_sync(0xffffffffu, n[0], which), TILE);
       const int within = at_tile - (before + __shfl_sync(0xffffffffu, sum - mine, which)) * heads;
       ic.head = within / ic.q.count;
       ic.i = within - ic.head * ic.q.count;
@@ -574,12 +576,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 }
 
 // Joins the parts of one sequence and query head (blockIdx.y): warps take parts in turn, lanes take columns.
-constexpr int kJoinWarps = 16;
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ PagedArgs a) {
+template <int D, int WARPS, bool BF16>
+__global__ void __launch_bounds__(WARPS * 32) join_kernel(const __grid_constant__ PagedArgs a) {
   constexpr int V = D / 32;
-  __shared__ float red[kJoinWarps][D];
-  __shared__ float2 sums[kJoinWarps];
+  __shared__ __align__(16) float red[WARPS][D];
+  __shared__ float2 sums[WARPS];
   ptx::wait_for_previous_kernel();
   ptx::allow_next_kernel();
   const int4 join = a.part.joins[blockIdx.x];
@@ -592,15 +593,15 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
     const long long slot = i == 0 ? join.z : 2ll * ((join.z >> 1) + i);
     return slot * a.h.rows + r;
   };
-  // kBatch parts in flight, with a running largest score
-  constexpr int kBatch = 8;
+  // kBatch parts of a warp in flight, with a running largest score
+  constexpr int kBatch = WARPS == 4 ? 4 : 5;
   float acc[V] = {}, sum = 0.f, most = -INFINITY;
-  for (int i0 = warp; i0 < join.w; i0 += kJoinWarps * kBatch) {
+  for (int i0 = warp; i0 < join.w; i0 += WARPS * kBatch) {
     float2 ml[kBatch];
     float x[kBatch][V];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = i0 + k * kJoinWarps;
+      const int i = i0 + k * WARPS;
       const long long row = row_of(min(i, join.w - 1));
       ml[k] = a.part.ml[row];
       const float* src = a.part.out + row * D + lane * V;
@@ -640,17 +641,21 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_cons
   if (lane == 0) sums[warp] = make_float2(most, sum);
   __syncthreads();
   if (threadIdx.x < D / 2) {
-    float top = -INFINITY;
+    // a lane has a warp's largest score and sum
+    const float2 its = lane < WARPS ? sums[lane] : make_float2(-INFINITY, 0.f);
+    float top = its.x;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, sums[w].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float total = 0.f, x = 0.f, y = 0.f;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float mine = exp2_fast(its.x - (top == -INFINITY ? 0.f : top));
+    float total = its.y * mine, x = 0.f, y = 0.f;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) {
-      const float scale = exp2_fast(sums[w].x - base);
-      total += sums[w].y * scale;
-      x += red[w][threadIdx.x * 2] * scale;
-      y += red[w][threadIdx.x * 2 + 1] * scale;
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+#pragma unroll 4
+    for (int w = 0; w < WARPS; ++w) {
+      const float scale = __shfl_sync(0xffffffffu, mine, w);
+      const float2 z = *reinterpret_cast<const float2*>(&red[w][threadIdx.x * 2]);
+      x += z.x * scale;
+      y += z.y * scale;
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     const int head = kv_head * a.h.group + sub * a.h.rows + r;
@@ -719,8 +724,12 @@ cudaError_t launch_typed(const PagedParams& p, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   e = launch_after(kernel, dim3(grid), kThreads, paged_smem_bytes<D>(), stream, 1, a);
   if (e != cudaSuccess || grid == 1) return e;
-  return launch_after(join_kernel<D, BF16>, dim3(static_cast<unsigned>(std::min<long long>(units, grid)), a.h.rows), kJoinWarps * 32,
-                      0, stream, 1, a);
+  // Few sequences have many parts (160 in flight in 32 warps), many have few, and then most of these CTAs find nothing to do:
+  // small ones come and go faster (16 warps everywhere: 64 sequences 114 us, 109 now; the window's 27.4, 24.5 now).
+  const bool many_parts = units * 8 <= grid;
+  const auto join = many_parts ? join_kernel<D, 32, BF16> : join_kernel<D, 4, BF16>;
+  return launch_after(join, dim3(static_cast<unsigned>(std::min<long long>(units, grid)), a.h.rows), many_parts ? 1024 : 128, 0,
+                      stream, 1, a);
 }
 
 }  // namespace
