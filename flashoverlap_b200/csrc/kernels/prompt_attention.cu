@@ -355,7 +355,7 @@ __device__ __forceinline__ void store_part(const PromptArgs& a, int index, int t
 // Joins the parts of a pair's rows, a warp for each row; lanes take columns.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ PromptArgs a) {
-  constexpr int V = D / 32, kBatch = 4;
+  constexpr int V = D / 32, kBatch = 6;
   ptx::wait_for_previous_kernel();
   ptx::allow_next_kernel();
   const PromptParams& p = a.p;
@@ -374,15 +374,32 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
     float y[kBatch][V];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int part = pair * a.parts + min(i0 + k, a.parts - 1);
+      ml[k] = make_float2(-INFINITY, 0.f);
+      if (i0 + k >= a.parts) continue;
+      const int part = pair * a.parts + i0 + k;
       const long long at = (static_cast<long long>(part) * 2 + tile) * kTileRows + row;
       ml[k] = a.part_ml[at];
       odd |= a.part_odd[part * 2 + tile] != 0;
-      // (a part that saw nothing has written no results)
-      const bool any = i0 + k < a.parts && (ml[k].x != -INFINITY || ml[k].y != 0.f);
-      if (!any) ml[k] = make_float2(-INFINITY, 0.f);
+      const float* src = a.part_out + at * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 z = *reinterpret_cast<const float4*>(src);
+        y[k][0] = z.x;
+        y[k][1] = z.y;
+        y[k][2] = z.z;
+        y[k][3] = z.w;
+      } else {
+        const float2 z = *reinterpret_cast<const float2*>(src);
+        y[k][0] = z.x;
+        y[k][1] = z.y;
+      }
+    }
 #pragma unroll
-      for (int v = 0; v < V; ++v) y[k][v] = any ? a.part_out[at * D + lane * V + v] : 0.f;
+    for (int k = 0; k < kBatch; ++k) {
+      // (a part that saw nothing has written no results)
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) y[k][v] = 0.f;
+      }
     }
     float top = most;
 #pragma unroll
