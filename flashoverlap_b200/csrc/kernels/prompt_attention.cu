@@ -19,9 +19,10 @@
 // A hidden token's weight is zero, and zero times infinity is not: in tiles that some row does not see whole, values behind
 // the length become zero, and should any other not be finite, the rows of the pair are computed one by one at the end.
 //
-// TMEM (512 columns of 32 bits): S_0, S_1 (128 each), O_0, O_1 (head_dim each); P_i, 16-bit pairs, over the first 64 of S_i
-// with a head_dim of 128, in columns of their own with 64.  Then the next scores need not wait for the products with the
-// weights, but only until the scores before have been read.
+// TMEM (512 columns of 32 bits): S_0, S_1 (128 each; P_i, 16-bit pairs, over the first 64 of S_i), O_0, O_1 (head_dim each).
+// Heads of 64 leave room for weights of their own, so that the next scores need not wait for the products; then both groups
+// of softmax warps ask for their powers at the same time and leave the unit idle at the same time (16384 tokens 377 us as it
+// is, 408 so).
 //
 // The running largest score of a row only moves when it grows by more than 8 (in powers of two): until then weights are up
 // to 2^8 instead of 1, which costs no accuracy (P is a floating-point type, sums are fp32), and O is not rescaled.
@@ -32,7 +33,7 @@
 // turn apart.  Long calls run at the power cap: 16384 tokens, 8 heads on 1, fp16, 494 us call after call (1.11 PFLOP/s, 0.82
 // of cuBLAS's sustained bf16 rate), 445 in a short burst.  2 x 4096 tokens, 32 heads on 8, window 1024, bf16: 145 to 160 us
 // (the cap again), ten tiles of keys for 8.3 that are seen, and 7000 clocks a pair for its first scores and its results.  3 x
-// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 35 us; 77 tokens: 7.7 a call.
+// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 33 us; 77 tokens: 7.7 a call.
 //
 // Tried and slower: two threads a row (16 warps of softmax; 16384 tokens 588 us), results stored by TMA or row by row, the
 // second half of the scores read again after the first weights have left, tiles multiplied and weighed by quarters.  A lane
@@ -113,7 +114,7 @@ constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
 constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
-                                                 // 64: 395 us, 418 with none; as many with a quarter)
+                                                 // 64: 418 us with none, 395; no other with a quarter)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
 
 template <int D>
@@ -125,16 +126,8 @@ constexpr int key_tile_bytes() {
   return kTileKeys * D * 2;
 }
 template <int D>
-constexpr bool weights_apart() {
-  return D == 64;
-}
-template <int D>
 constexpr int out_column(int tile) {
   return 2 * kTileKeys + tile * D;
-}
-template <int D>
-constexpr int weight_column(int tile) {
-  return weights_apart<D>() ? 2 * kTileKeys + 2 * D + tile * 64 : tile * kTileKeys;
 }
 constexpr int kStageBytes = 32 * 128;  // 64 columns of a warp's results, on their way out
 // shared memory behind the first 1024-byte boundary: two Q tiles, the ring, a stage for each softmax warp
@@ -441,7 +434,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   extern __shared__ __align__(128) uint8_t raw[];
   __shared__ __align__(16) uint4 answers[2];
   __shared__ __align__(8) uint64_t q_full[2], q_empty, kv_full[NB], kv_empty[NB], s_full[2], p_full[2][2], o_done[2], v_ok[kChecks],
-      checked[kPairsAhead], s_read[2], next_full[2], next_empty[2];
+      checked[kPairsAhead], next_full[2], next_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_pair[kPairsAhead];                           // the last pair (counted from 1) whose values are not all finite
   __shared__ int failed, unfinished, taken, pending, pairs[4];  // after a wait that ran out, see the end
@@ -456,7 +449,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       ptx::mbar_init(&p_full[i][0], kTileRows);
       ptx::mbar_init(&p_full[i][1], kTileRows);
       ptx::mbar_init(&o_done[i], 1);
-      ptx::mbar_init(&s_read[i], kTileRows);
       ptx::mbar_init(&next_full[i], 1);
       ptx::mbar_init(&next_empty[i], kReaders);
     }
@@ -615,7 +607,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
 #pragma unroll
       for (int y = 0; y < kTileKeys / 32; ++y) {
         const int x = half * (kTileKeys / 32) + y;
-        umma_f16_ts(tmem + out_column<D>(i), tmem + weight_column<D>(i) + x * 8, v + x * (16 * 128 / 16), idesc_o,
+        umma_f16_ts(tmem + out_column<D>(i), tmem + i * kTileKeys + x * 8, v + x * (16 * 128 / 16), idesc_o,
                     !first || x > 0);
       }
     };
@@ -653,22 +645,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
           ok = wait_warp(&kv_full[kbuf], buf.round & 1u);
           buf.next();
         }
-        if constexpr (weights_apart<D>()) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ok = ok && wait_warp(&s_read[i], tiles & 1u);
-            if (!ok || !more) continue;
-            ptx::tc_fence_after_sync();
-            if (elect_one()) {
-              scores(i, kbuf);
-              if (i == 1) {
-                ptx::umma_commit(&kv_empty[kbuf]);
-                if (j + 2 == r.n) ptx::umma_commit(&q_empty);
-              }
-            }
-            __syncwarp();
-          }
-        }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           // the first half of the products starts while the second half of the weights is computed
@@ -684,7 +660,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
             outputs(i, 1, vbuf, j == 0);
             ptx::umma_commit(&o_done[i]);
             if (i == 1) ptx::umma_commit(&kv_empty[vbuf]);
-            if (more && !weights_apart<D>()) {
+            if (more) {
               scores(i, kbuf);
               if (i == 1) {
                 ptx::umma_commit(&kv_empty[kbuf]);
@@ -742,7 +718,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     const int row = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes each, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * kTileKeys, t_o = tmem + lanes + out_column<D>(tile);
-    const uint32_t t_p = tmem + lanes + weight_column<D>(tile);
     const int token = row / a.group, head = row - token * a.group;
     const float c = a.scale_log2;
     uint32_t loaded = 0, tiles = 0;
@@ -767,10 +742,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         for (int q = 0; q < 4; ++q) ptx::tmem_ld_32x32b_x32(t_s + q * 32, s[q]);
 #pragma unroll
         for (int q = 0; q < 4; ++q) ptx::tmem_ld_wait_for(s[q]);
-        if constexpr (weights_apart<D>()) {
-          ptx::tc_fence_before_sync();
-          ptx::mbar_arrive(&s_read[tile]);
-        }
         if (masked) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -814,11 +785,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
             tmem_st_wait();
           }
         }
-        if (weights_apart<D>() && j > 0) {  // the weights before have been read
-          ok = wait_warp(&o_done[tile], (tiles - 1) & 1u);
-          if (!ok) break;
-          ptx::tc_fence_after_sync();
-        }
         float base = m == kLowest ? 0.f : m * c;
         base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
         const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
@@ -849,7 +815,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
             sum[e & 1] = add2(sum[e & 1], make_pair(y[e].x, y[e].y));
             w[g >> 2][(g & 3) * 8 + e] = pack<BF16>(y[e].x, y[e].y);
           }
-          if (g == 3 || g == 7) tmem_st_32x32b_x32(t_p + (g >> 2) * 32, w[g >> 2]);
+          if (g == 3 || g == 7) tmem_st_32x32b_x32(t_s + (g >> 2) * 32, w[g >> 2]);
           if (g == 3 || g == 7) {  // (the first half's way to TMEM is under the next weights)
             tmem_st_wait();
             ptx::tc_fence_before_sync();
