@@ -33,14 +33,13 @@
 // turn apart.  Long calls run at the power cap: 16384 tokens, 8 heads on 1, fp16, 494 us call after call (1.11 PFLOP/s, 0.82
 // of cuBLAS's sustained bf16 rate), 445 in a short burst.  2 x 4096 tokens, 32 heads on 8, window 1024, bf16: 145 to 160 us
 // (the cap again), ten tiles of keys for 8.3 that are seen, and 7000 clocks a pair for its first scores and its results.  3 x
-// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 33 us; 77 tokens: 7.7 a call.
+// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 32 us; 77 tokens: 7.7 a call.
 //
 // Tried and slower: two threads a row (16 warps of softmax; 16384 tokens 588 us), results stored by TMA or row by row, the
 // second half of the scores read again after the first weights have left, tiles multiplied and weighed by quarters.  A lane
 // that walks the tiles alone, and not its whole warp, takes 80 clocks to issue an instruction.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -114,7 +113,7 @@ constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
 constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
-                                                 // 64: 370 us; 396 with none, 387 with every fourth)
+                                                 // 64: 359 us; the others before the last step: 370, 396 with none, 387 with every fourth)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
 
 template <int D>
@@ -140,6 +139,7 @@ struct PromptArgs {
   PromptParams p;
   CUtensorMap q, k, v;
   int group, tokens;         // query heads of a head, tokens of a tile
+  FastDiv by_parts, by_row, by_kv, by_group;  // parts; batch * kv_heads; kv_heads; group
   int single;                // all CTAs fit the chip: there is nothing to take over
   // Few pairs of tiles: the keys of a pair are divided over `parts` CTAs, which leave unscaled results in fp32, for each row
   // the largest score (times log2 e) and the sum of weights, and for each tile whether a value was not finite.
@@ -245,13 +245,14 @@ __device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index
   PromptPair r;
   int part = 0;
   if (a.parts > 1) {
-    part = index % a.parts;
-    index /= a.parts;
+    const int pair = static_cast<int>(a.by_parts.div(index));
+    part = index - pair * a.parts;
+    index = pair;
   }
   // late tokens first: they see the most keys
   const int per = p.batch * p.kv_heads;
-  const int qb = index / per, rest = index - qb * per;
-  r.b = rest / p.kv_heads;
+  const int qb = static_cast<int>(a.by_row.div(index)), rest = index - qb * per;
+  r.b = static_cast<int>(a.by_kv.div(rest));
   r.kv_head = rest - r.b * p.kv_heads;
   r.t0 = (a.blocks - 1 - qb) * 2 * a.tokens;
   r.length = p.lengths == nullptr ? p.sk : min(max(__ldg(p.lengths + r.b), 0), p.sk);
@@ -260,7 +261,7 @@ __device__ __forceinline__ PromptPair prompt_pair(const PromptArgs& a, int index
   r.n = p0 < r.length ? r.tiles.count() : 0;  // 0: no row sees anything
   r.first = 0;
   if (a.parts > 1) {
-    const int per = (r.n + a.parts - 1) / a.parts;
+    const int per = static_cast<int>(a.by_parts.div(r.n + a.parts - 1));
     r.first = min(part * per, r.n);
     r.n = min(per, r.n - r.first);
   }
@@ -356,9 +357,10 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   const int rows = a.group * a.tokens;
   const int x = blockIdx.y * 8 + (threadIdx.x >> 5);  // rows of both tiles
   if (x >= 2 * rows) return;
-  const int tile = x / rows, row = x - tile * rows;
+  const int tile = x >= rows ? 1 : 0, row = x - tile * rows;
+  const int token = static_cast<int>(a.by_group.div(row));
   const PromptPair r = prompt_pair(a, pair * a.parts);
-  const int t = r.t0 + tile * a.tokens + row / a.group, head = r.kv_head * a.group + row % a.group;
+  const int t = r.t0 + tile * a.tokens + token, head = r.kv_head * a.group + row - token * a.group;
   if (t >= p.sq) return;
   bool odd = false;
   float acc[V] = {}, sum = 0.f, most = -INFINITY;
@@ -442,32 +444,39 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const uint32_t smem = (ptx::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = smem + 2 * kTileRows * D * 2, stage = ring + NB * TILE;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < 2; ++i) {
-      ptx::mbar_init(&q_full[i], 1);
-      ptx::mbar_init(&s_full[i], 1);
-      ptx::mbar_init(&p_full[i][0], kTileRows);
-      ptx::mbar_init(&p_full[i][1], kTileRows);
-      ptx::mbar_init(&o_done[i], 1);
-      ptx::mbar_init(&next_full[i], 1);
-      ptx::mbar_init(&next_empty[i], kReaders);
+  if (lane == 0 && warp < 4) {  // (a barrier at a time by one thread takes 600 clocks)
+    if (warp == 0) {
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&q_full[i], 1);
+        ptx::mbar_init(&s_full[i], 1);
+        ptx::mbar_init(&p_full[i][0], kTileRows);
+        ptx::mbar_init(&p_full[i][1], kTileRows);
+        ptx::mbar_init(&o_done[i], 1);
+      }
+    } else if (warp == 1) {
+      for (int i = 0; i < NB; ++i) {
+        ptx::mbar_init(&kv_full[i], 1);
+        ptx::mbar_init(&kv_empty[i], 1);
+      }
+      ptx::mbar_init(&q_empty, 1);
+    } else if (warp == 2) {
+      for (int i = 0; i < kChecks; ++i) ptx::mbar_init(&v_ok[i], 2);
+      failed = 0;
+      unfinished = INT32_MAX;
+      taken = 0;
+      pending = -1;
+    } else {
+      for (int i = 0; i < kPairsAhead; ++i) {
+        ptx::mbar_init(&checked[i], 2);
+        odd_pair[i] = 0;
+      }
+      for (int i = 0; i < 2; ++i) {
+        ptx::mbar_init(&next_full[i], 1);
+        ptx::mbar_init(&next_empty[i], kReaders);
+      }
     }
-    for (int i = 0; i < NB; ++i) {
-      ptx::mbar_init(&kv_full[i], 1);
-      ptx::mbar_init(&kv_empty[i], 1);
-    }
-    for (int i = 0; i < kChecks; ++i) ptx::mbar_init(&v_ok[i], 2);
-    for (int i = 0; i < kPairsAhead; ++i) {
-      ptx::mbar_init(&checked[i], 2);
-      odd_pair[i] = 0;
-    }
-    ptx::mbar_init(&q_empty, 1);
     ptx::mbar_fence_init();
     ptx::fence_proxy_async_smem();
-    failed = 0;
-    unfinished = INT32_MAX;
-    taken = 0;
-    pending = -1;
   }
   if (warp == 8) {
     if (lane == 0) {
@@ -718,7 +727,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
     const int row = threadIdx.x & 127;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 lanes each, in the upper half of an address
     const uint32_t t_s = tmem + lanes + tile * kTileKeys, t_o = tmem + lanes + out_column<D>(tile);
-    const int token = row / a.group, head = row - token * a.group;
+    const int token = static_cast<int>(a.by_group.div(row)), head = row - token * a.group;
     const float c = a.scale_log2;
     uint32_t loaded = 0, tiles = 0;
     bool ok = true;
@@ -1001,8 +1010,7 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
     const long long grid = std::min<long long>((rows + 7) / 8, 8ll * device_sm_count());
     return launch_after(prompt_rows_kernel<D, BF16>, dim3(static_cast<unsigned>(grid)), 256, 0, stream, 1, p);
   }
-  PromptArgs a;
-  std::memset(&a, 0, sizeof(a));
+  PromptArgs a{};
   a.p = p;
   a.group = p.heads / p.kv_heads;
   const PromptGrid g = prompt_grid(p);
@@ -1024,6 +1032,10 @@ cudaError_t launch_typed(const PromptParams& p, DType dt, cudaStream_t stream) {
   }
   const long long grid = g.pairs * g.parts;
   a.single = grid <= device_sm_count();
+  a.by_parts = FastDiv(static_cast<uint32_t>(a.parts));
+  a.by_row = FastDiv(static_cast<uint32_t>(p.batch * p.kv_heads));
+  a.by_kv = FastDiv(static_cast<uint32_t>(p.kv_heads));
+  a.by_group = FastDiv(static_cast<uint32_t>(a.group));
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   if (a.parts > 1) {
     char* ws = static_cast<char*>(p.workspace);
