@@ -105,3 +105,34 @@ def test_what_a_pool_refuses():
     assert pool.free_pages() == 1 and pool.pages(b)[0] not in (pool.pages(pool.add(1)),)
     with pytest.raises(RuntimeError):
         pool.free(a)
+
+
+def test_what_a_cache_refuses_before_it_takes_memory():
+    from flashoverlap_b200.models import PagedKVCache
+
+    for kw in (dict(device="cpu"), dict(head_dim=12), dict(head_dim=0), dict(kv_heads=0), dict(page_size=0)):
+        args = dict(pages=4, page_size=16, kv_heads=2, head_dim=64, device="cuda:0")
+        args.update(kw)
+        with pytest.raises(ValueError):
+            PagedKVCache(**args)
+
+
+def test_pages_of_a_forked_tree():
+    # a page lives until the last sequence that holds it has ended, in whatever order they end
+    pool = Pool(20, 4)
+    root = pool.add(8)
+    leaves = [pool.fork(root)[0] for _ in range(5)]
+    assert pool.free_pages() == 18 and all(pool.pages(s) == pool.pages(root) for s in leaves)
+    pool.grow(leaves, [1] * 5)
+    assert pool.free_pages() == 13 and len({pool.pages(s)[-1] for s in leaves}) == 5
+    pool.free(root)
+    assert pool.free_pages() == 13
+    moves = pool.compact()
+    assert moves.shape[0] == 0
+    for s in leaves[:-1]:
+        pool.free(s)
+    assert pool.free_pages() == 17
+    moves = pool.compact().tolist()
+    assert all(t < 3 <= f for f, t in moves) and sorted(pool.pages(leaves[-1])) == [0, 1, 2]
+    again, copied = pool.fork(leaves[-1])
+    assert copied.tolist() == [[pool.pages(leaves[-1])[2], pool.pages(again)[2]]]
