@@ -684,13 +684,14 @@ int grid_size(const PagedParams& p) {
 // Few tiles for each sequence and head: a cluster of CTAs takes them, joins in its shared memory and needs neither
 // workspace nor a second kernel.  Returns the CTAs of a cluster, 0 for the general form.  Up to eight tiles a CTA where the
 // clusters fill at least half of the chip's places, else up to two: 32 sequences of 256 tokens on 8 heads of 128 take 7.2 us
-// (10.3 in the general form), 8 of 2048 13.0 (15.0), one of 1024 6.2 (7.2), one of 4096 would 11.9 (9.0).  Longer ones go
+// (10.3 in the general form), 8 of 2048 13.0 (15.0), one of 1024 6.2 (7.2), one of 4096 would 11.9 (9.0).  In up to two waves: 64
+// sequences of up to 512 tokens 20.9 (23.4); with 128 of 256 tokens there is no difference, 256 would lose.  Longer ones go
 // the general way although equal lengths would not lose: it does not depend on them.
 int short_cluster(const PagedParams& p) {
   const long long units = unit_count(p), tiles = most_tiles(p), slots = static_cast<long long>(kCtasPerSm) * device_sm_count();
   int c = 1;
   while (c < kMaxCluster && c < tiles && units * c * 2 <= slots) c *= 2;
-  return units * c <= slots && (tiles + c - 1) / c <= (units * c * 2 >= slots ? 8 : 2) ? c : 0;
+  return (units * c <= slots || units <= 2 * slots) && (tiles + c - 1) / c <= (units * c * 2 >= slots ? 8 : 2) ? c : 0;
 }
 
 template <int D, bool BF16>
