@@ -592,6 +592,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         ptx::mbar_arrive(&next_empty[slot]);
         if (index < 0) break;
       }
+      // (a join that waits on the SMs takes longer than one that comes when they are free)
+      if (a.parts == 1) ptx::allow_next_kernel();
     }
     __syncwarp();
   } else if (warp == 9) {
