@@ -41,6 +41,8 @@ class TPDecoderBlock(nn.Module):
         self.heads = n_heads // ws
         self.kv_heads = max(1, n_kv_heads // ws)
         self.window, self.sinks = window, sinks
+        if window and self.head_dim not in (64, 128):
+            raise ValueError(f"attention in a window takes heads of 64 or 128 values, not {self.head_dim}")
         dev = device if device is not None else torch.device("cuda", torch.cuda.current_device())
         g = torch.Generator(device="cpu").manual_seed(seed * 1000 + self.rank)
 

@@ -679,3 +679,17 @@ def test_a_split_prompt_in_two_graphs():
                 g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def test_decoder_block_refuses_heads_that_the_kernels_do_not_take():
+    from flashoverlap_b200.models import PagedKVCache
+    from flashoverlap_b200.models.decoder_block import TPDecoderBlock
+
+    with pytest.raises(ValueError, match="heads of 64 or 128"):
+        TPDecoderBlock(None, 512, 256, 2, 2, window=10)
+    block = TPDecoderBlock(None, 512, 256, 2, 2)      # heads of 256: prompts as before, no cache
+    cache = PagedKVCache(4, 16, 2, 256)
+    x = torch.zeros(1, 512, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="heads of 64 or 128"):
+        block.decode(x, x, cache, [cache.add()])
+    assert cache.pool.free_pages() == 4
