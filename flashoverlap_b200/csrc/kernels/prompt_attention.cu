@@ -111,7 +111,6 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const __grid_constant_
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
-constexpr float kLowest = -3.4028234663852886e38f;  // the largest score of a row that has seen nothing
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
                                                  // 64: 359 us; the others before the last step: 370, 396 with none, 387 with every fourth)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
@@ -323,7 +322,7 @@ __device__ __forceinline__ void store_part(const PromptArgs& a, int index, int t
                                            bool any, bool odd, float m, float l) {
   const int lane = row & 31;
   const long long first = (static_cast<long long>(index) * 2 + tile) * kTileRows;
-  a.part_ml[first + row] = any && m != kLowest ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
+  a.part_ml[first + row] = any && m != -INFINITY ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
   if (row == 0) a.part_odd[index * 2 + tile] = odd;
   if (!any) return;
 #pragma unroll
@@ -741,7 +740,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       const bool real = token < a.tokens && t < p.sq;
       const int last = real && pos < r.length ? pos : -1;  // the last visible token
       const int lo = p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0;
-      float m = kLowest, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // the first score that is seen raises m, however small the scale is
       for (int j = 0; j < r.n; ++j, ++tiles) {
         const int first_key = r.key(j);
         const bool masked = !sees_whole(a, r, tile, first_key);
@@ -774,7 +773,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         top[0] = max3_nan(top[0], __uint_as_float(s[0][31]), __uint_as_float(s[1][31]));
         top[1] = max3_nan(top[1], __uint_as_float(s[2][31]), __uint_as_float(s[3][31]));
         const float most = max3_nan(max3_nan(top[0], top[1], m), top[2], top[3]);
-        const bool raise = real && !((most - m) * c <= kRaise);  // also for NaN; rows that no token fills hold anything
+        // also for NaN; a row that has seen nothing stays as it is; rows that no token fills hold anything
+        const bool raise = real && most != m && !((most - m) * c <= kRaise);
         if (__any_sync(0xffffffffu, raise)) {
           const float factor = raise ? exp2_fast((m - most) * c) : 1.f;
           if (raise) m = most;
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
             tmem_st_wait();
           }
         }
-        float base = m == kLowest ? 0.f : m * c;
+        float base = m == -INFINITY ? 0.f : m * c;
         base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
         const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
         Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
