@@ -4,8 +4,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
 
+#include <atomic>
 #include <cmath>
+#include <cstring>
 #include <limits>
+#include <mutex>
 #include <unordered_set>
 
 #include "../kernels/attention.h"
@@ -106,7 +109,54 @@ void check_table(const at::Tensor& table, int64_t seqs, const PageLayout& l, con
               "page_table covers more than 2^31 - 1024 tokens");
 }
 
+// What the prompt kernel reports of waits that ran out: a word for each device, in host memory that all devices see under
+// its own address, read before each call without waiting for anything.  Allocated at the first call, also where that is being captured, and kept.
+constexpr int kStatusDevices = 64;
+std::atomic<StatusWord*> status_words{nullptr};
+std::atomic<int64_t> prompt_wait_ns{10000000000};
+
+StatusWord* status_of(int device) {
+  TORCH_CHECK(device >= 0 && device < kStatusDevices, "attention: device number out of range");
+  static std::mutex mu;
+  if (status_words.load(std::memory_order_acquire) == nullptr) {
+    std::lock_guard<std::mutex> lock(mu);
+    if (status_words.load() == nullptr) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the allocation is no part of a graph
+      check_launch(cudaThreadExchangeStreamCaptureMode(&mode), "attention: status");
+      void* words = nullptr;
+      const size_t bytes = kStatusDevices * sizeof(StatusWord);
+      const cudaError_t e = cudaHostAlloc(&words, bytes, cudaHostAllocMapped | cudaHostAllocPortable);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      check_launch(e, "attention: status");
+      std::memset(words, 0, bytes);
+      status_words.store(static_cast<StatusWord*>(words), std::memory_order_release);
+    }
+  }
+  return status_words.load() + device;
+}
+void check_previous(StatusWord* word, const char* op) {
+  const volatile StatusWord* s = word;
+  TORCH_CHECK(s->code == ST_OK, op, ": a wait of an earlier call of prompt_attention on this device ran out (warp ", s->where,
+              " of CTA ", s->seen, "); rows that it had not finished are NaN (attention_reset() clears the state)");
+}
+
 }  // namespace
+
+// {code, warp, CTA} of what has been reported for a device since the last reset; code 0: nothing.  Does not wait.
+static std::vector<int64_t> attention_status_op(int64_t device) {
+  if (status_words.load() == nullptr) return {ST_OK, 0, 0};
+  const volatile StatusWord* s = status_of(static_cast<int>(device));
+  return {s->code, s->where, s->seen};
+}
+static void attention_reset_op(int64_t device) {
+  if (status_words.load() == nullptr) return;
+  std::memset(status_of(static_cast<int>(device)), 0, sizeof(StatusWord));
+}
+// Limit of the waits in kernels launched from now on; returns the one before.
+static int64_t attention_set_timeout_ns_op(int64_t ns) {
+  TORCH_CHECK(ns >= 0 && ns <= 3600000000000, "timeout must be at most an hour");
+  return prompt_wait_ns.exchange(ns);
+}
 
 // out[b, t, h] of q [batch, sq, heads, head_dim], k and v [batch, sk, kv_heads, head_dim]; see attention.h.
 static void prompt_attention_op(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, int64_t window, int64_t sinks,
@@ -156,6 +206,9 @@ static void prompt_attention_op(at::Tensor q, at::Tensor k, at::Tensor v, at::Te
   p.sinks = static_cast<int>(sinks);
   p.scale = scale_or(scale, dim);
   c10::cuda::CUDAGuard guard(q.device());
+  p.status = status_of(q.get_device());
+  check_previous(p.status, "prompt_attention");
+  p.wait_ns = static_cast<unsigned long long>(prompt_wait_ns.load());
   // from the caching allocator, for this call alone: calls on other streams and captured graphs have their own
   at::Tensor workspace;
   if (const size_t bytes = prompt_workspace_bytes(p)) {
@@ -366,6 +419,9 @@ TORCH_LIBRARY_FRAGMENT(flashoverlap_op, m) {
   m.def("paged_attention_new", &fo::paged_attention_new_op);
   m.def("cache_append", &fo::cache_append_op);
   m.def("copy_pages", &fo::copy_pages_op);
+  m.def("attention_status", &fo::attention_status_op);
+  m.def("attention_reset", &fo::attention_reset_op);
+  m.def("attention_set_timeout_ns", &fo::attention_set_timeout_ns_op);
   m.def("page_place", &fo::page_place_op);
   m.def("seen_tiles", &fo::seen_tiles_op);
 }

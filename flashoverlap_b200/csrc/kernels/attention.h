@@ -96,6 +96,10 @@ struct PromptParams {
   int window, sinks;
   float scale;
   void* workspace;  // prompt_workspace_bytes(), 16-byte aligned, contents arbitrary
+  // Limit of each wait inside the kernel.  A CTA whose wait runs out writes `status` (mapped host memory, ST_TIMEOUT_PIPE, the
+  // warp that gave up and the CTA) and makes the rows that it has taken and not finished NaN.
+  unsigned long long wait_ns;
+  StatusWord* status;
 };
 size_t prompt_workspace_bytes(const PromptParams& p);
 // head_dim 64 or 128, heads a multiple of kv_heads (at most 128 times), sq <= sk; addresses and strides in whole 16 bytes.

@@ -110,7 +110,6 @@ __global__ void __launch_bounds__(256) prompt_rows_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kTileRows = 128, kTileKeys = 128;
 constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
-constexpr uint64_t kDeadlineNs = 10000000000ull;  // of a wait; the longest, for rows computed one by one, are below a second
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
                                                  // 64: 359 us; the others before the last step: 370, 396 with none, 387 with every fourth)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
@@ -438,7 +437,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
       checked[kPairsAhead], next_full[2], next_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int odd_pair[kPairsAhead];                           // the last pair (counted from 1) whose values are not all finite
-  __shared__ int failed, unfinished, taken, pending, pairs[4];  // after a wait that ran out, see the end
+  __shared__ int failed, unfinished, taken, pending, pairs[4];  // after a wait that ran out (by warp `failed` - 1), see the end
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t smem = (ptx::smem_u32(raw) + 1023u) & ~1023u;
   const uint32_t ring = smem + 2 * kTileRows * D * 2, stage = ring + NB * TILE;
@@ -493,17 +492,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   const uint32_t tmem = tmem_slot;
   ptx::wait_for_previous_kernel();
 
-  // Each wait has a limit of its own: a CTA may work for long.  Once one has run out, all give up.
+  // Each wait has a limit of its own: a CTA may work for long.  Once one has run out, all give up.  (The clock is looked at
+  // every 1024th time; where the limit is short, which it is in tests, each time, and the thread is not suspended, for a
+  // microsecond or more, between looks.)
+  const bool brief = p.wait_ns < 1000000ull;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
+    if (!brief && ptx::mbar_try_wait(bar, parity)) return true;
     uint64_t deadline = 0;
     for (uint32_t tries = 1;; ++tries) {
-      if (ptx::mbar_try_wait(bar, parity)) return true;
-      if ((tries & 0x3ffu) == 0u) {
+      if (brief ? ptx::mbar_test_wait(bar, parity) : ptx::mbar_try_wait(bar, parity)) return true;
+      if (brief || (tries & 0x3ffu) == 0u) {
         const uint64_t now = ptx::globaltimer_ns();
-        if (deadline == 0) deadline = now + kDeadlineNs;
-        if (now > deadline || *const_cast<volatile int*>(&failed) != 0) {
-          *const_cast<volatile int*>(&failed) = 1;
+        if (deadline == 0) deadline = now + p.wait_ns;
+        if (*const_cast<volatile int*>(&failed) != 0) return false;
+        if (now > deadline) {
+          *const_cast<volatile int*>(&failed) = warp + 1;
           return false;
         }
       }
@@ -909,8 +912,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
   }
   __syncthreads();
   if (*const_cast<volatile int*>(&failed) != 0) {
-    // A wait ran out: copies, answers and products that are still under way get time to end before their memory is given
-    // back, and the rows of all pairs that this CTA has taken and not finished become NaN.
+    // A wait ran out: the host is told, copies, answers and products that are still under way get time to end before their
+    // memory is given back, and the rows of all pairs that this CTA has taken and not finished become NaN.
+    if (threadIdx.x == 0) {  // details first, the code last; of several CTAs any may be the one that is read
+      volatile StatusWord* status = p.status;
+      status->where = static_cast<uint32_t>(failed - 1);
+      status->seen = blockIdx.x;
+      __threadfence_system();
+      status->code = ST_TIMEOUT_PIPE;
+      __threadfence_system();
+    }
     const uint64_t until = ptx::globaltimer_ns() + 2000000ull;
     while (ptx::globaltimer_ns() < until) __nanosleep(1000);
     __syncthreads();

@@ -1,5 +1,8 @@
 """Functional wrappers over the native operators."""
 from .attention import (  # noqa: F401
+    attention_reset,
+    attention_set_timeout_ms,
+    attention_status,
     cache_append,
     copy_pages,
     paged_attention,

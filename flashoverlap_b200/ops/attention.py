@@ -10,6 +10,10 @@ A cache is ``[pages, 2, kv_heads, page_size, head_dim]``, keys at 0 and values a
 ``j % page_size``.  Page numbers and lengths stay on the GPU and are not read by the host; the kernels check them.
 
 Forward only: tensors that require a gradient are refused unless gradients are off.
+
+The waits inside the prompt's kernel have a limit (``attention_set_timeout_ms``, 10 s by default).  One that runs out makes
+the rows that its part of the work had not finished NaN, and is reported: later calls of ``prompt_attention`` on that device
+raise, and ``attention_status`` says so, until ``attention_reset``.
 """
 from __future__ import annotations
 
@@ -34,6 +38,32 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: 
         return torch.ops.flashoverlap_op.prompt_attention_new.default(q, k, v, window, sinks, lengths, scale)
     torch.ops.flashoverlap_op.prompt_attention.default(q, k, v, out, window, sinks, lengths, scale)
     return out
+
+
+def _device_index(device) -> int:
+    index = None if device is None else torch.device(device).index
+    return torch.cuda.current_device() if index is None else index
+
+
+def attention_status(device=None) -> str:
+    """Waits for the device; "ok", or what ``prompt_attention`` has reported on it since the last ``attention_reset``."""
+    index = _device_index(device)
+    torch.cuda.synchronize(index)
+    code, warp, cta = torch.ops.flashoverlap_op.attention_status.default(index)
+    return "ok" if code == 0 else f"a wait ran out [code {code}, warp {warp} of CTA {cta}]"
+
+
+def attention_reset(device=None) -> None:
+    """Waits for the device and forgets what has been reported on it."""
+    index = _device_index(device)
+    torch.cuda.synchronize(index)
+    torch.ops.flashoverlap_op.attention_reset.default(index)
+
+
+def attention_set_timeout_ms(ms: float) -> float:
+    """Limit of a wait in kernels launched from now on (a captured graph keeps the one of its capture); returns the one
+    before."""
+    return torch.ops.flashoverlap_op.attention_set_timeout_ns.default(round(ms * 1e6)) / 1e6
 
 
 def paged_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
