@@ -91,3 +91,30 @@ print("right")
 """ % str(__import__("pathlib").Path(__file__).resolve().parents[1])
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "right" in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_one_by_one_take_longer_than_a_wait_may(timeout, dim):
+    # The last tiles of the first sequence hold a value that is not finite: their rows are computed one by one, 32 a warp over
+    # some 4000 tokens, tens of milliseconds, while the other warps wait for the pair that the CTA has claimed.
+    batch, n, kv, bad = 8, 4096, 10, 4000
+    q, k, v = (randn(batch, n, kv, dim, dtype=BF16, seed=i) for i in range(3))
+    clean = ops.prompt_attention(q, k, v)
+    check_prompt(q[:1], k[:1], v[:1], clean[:1], heads=(0,))
+    v[0, bad, :, 1] = float("inf")
+    start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+
+    def call():
+        start.record()
+        out = ops.prompt_attention(q, k, v)
+        end.record()
+        return out
+
+    got = timeout(3_000_000, call)
+    assert ops.attention_status() == "ok"
+    assert start.elapsed_time(end) > 10        # else nothing here has waited for long
+    hit = torch.zeros(batch, n, dtype=torch.bool, device="cuda")
+    hit[0, bad:] = True
+    assert not got[hit][..., 1].isfinite().any()
+    assert torch.equal(got[1:], clean[1:]) and torch.equal(got[0, :3840], clean[0, :3840])
+    check_prompt(q[:1, :bad], k[:1, :bad], v[:1, :bad], got[:1, :bad], heads=(0, 9))
