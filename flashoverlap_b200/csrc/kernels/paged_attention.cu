@@ -36,6 +36,10 @@ constexpr int kRows = 16;      // query heads that one pass serves
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCluster = 8;
 constexpr int kAhead = 4;      // lengths that a lane asks for at a time
+// Powers of two in the weights: fp16 has numbers from 2^-24 to 2^16, and a weight of 2^-25 of the largest would vanish from the
+// products and not from the sum; 10^5 of them are more than a step of the result.
+template <bool BF16>
+constexpr float kFactor = BF16 ? 0.f : 15.f;
 constexpr int kStages = 3;     // of a warp's ring, 8 KB each (two CTAs then take all of an SM's shared memory)
 
 // Tokens of a warp and of a CTA.  8 KB of keys and values either way: with 16 tokens of 64 values, what a warp does for every
@@ -387,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float base = top == -INFINITY ? 0.f : top * a.scale_log2;
+        const float base = top == -INFINITY ? 0.f : top * a.scale_log2, shift = kFactor<BF16> - base;
         alpha[nt][x] = exp2_fast(m[nt][x] * a.scale_log2 - base);
         raised |= top != m[nt][x];
         m[nt][x] = top;
@@ -397,12 +401,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attention_kernel(c
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             float& w = c[t][nt][e * 2 + x];
-            w = exp2_fast(w * a.scale_log2 - base);
+            w = exp2_fast(w * a.scale_log2 + shift);
             l[nt][x] += w;
           }
         }
       }
-      // weights are rounded to the type of the values, as the tensor cores take them; their sum is not
+      // weights are rounded to the type of the values, as the tensor cores take them; their sum, which has the same factor, is not
 #pragma unroll
       for (int t = 0; t < TOK / 16; ++t) {
         pf[t][nt][0] = transpose_8x8(pack<BF16>(c[t][nt][0], c[t][nt][1]));

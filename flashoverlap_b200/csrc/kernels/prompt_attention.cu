@@ -26,7 +26,9 @@
 // is, 408 so).
 //
 // The running largest score of a row only moves when it grows by more than 8 (in powers of two): until then weights are up
-// to 2^8 instead of 1, which costs no accuracy (P is a floating-point type, sums are fp32), and O is not rescaled.
+// to 2^8 instead of 1, which costs no accuracy (P is a floating-point type, sums are fp32), and O is not rescaled.  In fp16,
+// which has numbers from 2^-24 to 2^16, weights and their sum carry a factor of 2^7 besides: a weight of 2^-25 of the largest
+// would vanish from P and not from the sum, and 10^5 of them are more than a step of the result.
 //
 // What bounds it: a tile of keys takes a pair 2950 clocks (head_dim 128), 2048 of them tensor work.  The 128 weights of a
 // thread take some 1700 (200 until the scores are in registers, 300 for the largest, 1250 for powers, sums and their way to
@@ -114,6 +116,8 @@ constexpr int kSoftmaxThreads = 256, kPromptThreads = 384;
 constexpr int kPolyEvery = 8;                    // every eighth pair of weights comes from the polynomial (16384 tokens, heads of
                                                  // 64: 359 us; the others before the last step: 370, 396 with none, 387 with every fourth)
 constexpr float kRaise = 8.f;                    // powers of two that a row's largest score may grow before O is rescaled
+template <bool BF16>
+constexpr float kFactor = BF16 ? 0.f : 7.f;      // powers of two in the weights: at most 2^(8 + 7) of fp16's 2^16
 
 template <int D>
 constexpr int ring_buffers() {
@@ -805,7 +809,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_attention_kernel(con
         }
         float base = m == -INFINITY ? 0.f : m * c;
         base += base - base;  // NaN if the largest score is infinite: the polynomial would hide it
-        const Pair c2 = make_pair(c, c), base2 = make_pair(-base, -base);
+        const float shift = kFactor<BF16> - base;
+        const Pair c2 = make_pair(c, c), base2 = make_pair(shift, shift);
         Pair sum[2] = {make_pair(0.f, 0.f), make_pair(0.f, 0.f)};
         // Eight pairs at a time: their arguments, their powers, then what is done with them, so that nothing waits for the
         // power just asked for.

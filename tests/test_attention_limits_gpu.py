@@ -39,3 +39,39 @@ def test_scores_near_the_lowest_number():
         q[..., 0] = -255 / 128 * 2.0 ** 64
         k[..., 0] = steps[torch.arange(sk) % 7 // 3 % 2].cuda()[None, :, None]
         check_prompt(q, k, v, ops.prompt_attention(q, k, v, scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_small_weights_of_half_precision(dim):
+    # Every 16th token has weight 1 and value 0, the others weight 2^-26.5, which is no number of fp16, and value 2^15: the
+    # small weights are all of the result.  They are kept with a factor of at least 2^7, next to which an absolute error of
+    # 2^-25 is 2^-5.5 of them; then half a step for the weights and half for the result, and the errors of the oracle's bound
+    # that are not fp16's (scores of at most 18.4).
+    t, big = 18.375, 2.0 ** 15
+    delta = 18.4 * (dim + 4) * 2.0 ** -23 + 2.0 ** -21
+    for batch, sq, sk, heads, kv in SHAPES + [(1, 1000, 2500, 8, 4)]:
+        q, k, v = (torch.zeros(batch, n, h, dim, dtype=FP16, device="cuda") for n, h in ((sq, heads), (sk, kv), (sk, kv)))
+        q[..., 0] = 1
+        k[:, ::16, :, 0] = t
+        v[:], v[:, ::16] = big, 0
+        seen = torch.arange(sk - sq + 1, sk + 1, dtype=torch.float64, device="cuda")
+        large = torch.ceil(seen / 16)
+        small = (seen - large) * torch.exp(torch.tensor(-t, dtype=torch.float64))
+        want = big * small / (large + small)
+        got = ops.prompt_attention(q, k, v, scale=1.0)
+        tol = want * (2.0 ** -5.5 + 2.0 ** -10 + 2 * delta + sk * 2.0 ** -23) + 2.0 ** -25
+        assert ((got.double() - want[None, :, None, None]).abs() <= tol[None, :, None, None]).all()
+    for lengths in ([200, 17], [6000, 5000]):
+        p = Paged(lengths, 1, dim, 16, FP16)
+        p.cache.zero_()
+        p.cache[:, 0, :, 0, 0] = t
+        p.cache[:, 1, :, 1:] = big
+        q = torch.zeros(2, 4, dim, dtype=FP16, device="cuda")
+        q[..., 0] = 1
+        got = ops.paged_attention(q, p.cache, p.table, p.lengths, scale=1.0)
+        for s, n in enumerate(lengths):
+            large = -(-n // 16)
+            small = (n - large) * torch.exp(torch.tensor(-t, dtype=torch.float64)).item()
+            want = big * small / (large + small)
+            tol = want * (2.0 ** -5.5 + 2.0 ** -10 + 2 * delta + n * 2.0 ** -23) + 2.0 ** -25
+            assert (got[s].double() - want).abs().max() <= tol, (n, want, got[s])
