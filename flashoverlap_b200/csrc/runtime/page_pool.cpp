@@ -42,6 +42,10 @@ int PagePool::Take() {
   return page;
 }
 
+void PagePool::Give(int page) {
+  if (--users_[static_cast<size_t>(page)] == 0) free_.push_back(page);
+}
+
 int64_t PagePool::Add(int64_t length) {
   TORCH_CHECK(length >= 0 && length <= kMostTokens, "PagePool: length out of range");
   const int64_t need = PagesFor(length);
@@ -71,6 +75,28 @@ void PagePool::Grow(std::vector<int64_t> seqs, std::vector<int64_t> counts) {
   }
 }
 
+void PagePool::Shrink(std::vector<int64_t> seqs, std::vector<int64_t> counts) {
+  TORCH_CHECK(seqs.size() == counts.size(), "PagePool: as many counts as sequences");
+  std::set<int64_t> seen;
+  for (size_t i = 0; i < seqs.size(); ++i) {
+    const Sequence& s = At(seqs[i]);
+    TORCH_CHECK(seen.insert(seqs[i]).second, "PagePool: sequence ", seqs[i], " is named twice");
+    TORCH_CHECK(counts[i] >= 0 && counts[i] <= s.length, "PagePool: count out of range");
+    const int64_t length = s.length - counts[i];
+    TORCH_CHECK(counts[i] == 0 || length % page_size_ == 0 ||
+                    users_[static_cast<size_t>(s.pages[static_cast<size_t>(length / page_size_)])] == 1,
+                "PagePool: sequence ", seqs[i], " would end inside a page that it shares");
+  }
+  for (size_t i = seqs.size(); i-- > 0;) {
+    Sequence& s = sequences_.find(seqs[i])->second;
+    s.length -= counts[i];
+    while (static_cast<int64_t>(s.pages.size()) > PagesFor(s.length)) {
+      Give(s.pages.back());
+      s.pages.pop_back();
+    }
+  }
+}
+
 std::tuple<int64_t, at::Tensor> PagePool::Fork(int64_t seq) {
   Sequence copy = At(seq);
   std::vector<std::pair<int, int>> moves;
@@ -88,9 +114,7 @@ std::tuple<int64_t, at::Tensor> PagePool::Fork(int64_t seq) {
 
 void PagePool::Free(int64_t seq) {
   const Sequence& s = At(seq);
-  for (auto it = s.pages.rbegin(); it != s.pages.rend(); ++it) {
-    if (--users_[static_cast<size_t>(*it)] == 0) free_.push_back(*it);
-  }
+  for (auto it = s.pages.rbegin(); it != s.pages.rend(); ++it) Give(*it);
   sequences_.erase(seq);
 }
 
@@ -154,6 +178,7 @@ TORCH_LIBRARY_FRAGMENT(flashoverlap_class, m) {
       .def(torch::init<int64_t, int64_t>())
       .def("add", &PagePool::Add)
       .def("grow", &PagePool::Grow)
+      .def("shrink", &PagePool::Shrink)
       .def("fork", &PagePool::Fork)
       .def("free", &PagePool::Free)
       .def("compact", &PagePool::Compact)

@@ -21,6 +21,10 @@ class PagePool : public torch::CustomClassHolder {
   int64_t Add(int64_t length);
   // Tokens behind the last ones: sequence seqs[i] becomes counts[i] longer.  All of them or none.
   void Grow(std::vector<int64_t> seqs, std::vector<int64_t> counts);
+  // Takes back the last counts[i] tokens of sequence seqs[i], and the pages behind them.  All of them or none; a sequence does
+  // not come to end inside a page that it shares, which its next tokens would change for the others.  What Grow has just done
+  // is undone to the last free page.
+  void Shrink(std::vector<int64_t> seqs, std::vector<int64_t> counts);
   // A new sequence with the tokens of another, and the page that has to be copied for it ([n, 2] int32, n 0 or 1).
   std::tuple<int64_t, at::Tensor> Fork(int64_t seq);
   void Free(int64_t seq);
@@ -45,6 +49,7 @@ class PagePool : public torch::CustomClassHolder {
   const Sequence& At(int64_t seq) const;
   int64_t PagesFor(int64_t length) const { return (length + page_size_ - 1) / page_size_; }
   int Take();
+  void Give(int page);
   int64_t page_size_, next_ = 0;
   std::vector<int> free_;   // the last one is taken first
   std::vector<int> users_;  // sequences that hold a page

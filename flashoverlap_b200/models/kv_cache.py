@@ -19,11 +19,13 @@ class PagedKVCache:
     sequences.  Everything on the GPU goes to the current stream: pages that ``free`` gives back may be written by what
     comes later in that stream, so a cache is used from one stream, or the streams are ordered by the caller.
 
-    An operation that needs more pages than are free raises RuntimeError and leaves the cache as it was."""
+    An operation that is refused, for want of pages or for what it is given, raises and leaves the cache as it was."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype=torch.bfloat16, device=None):
         if kv_heads < 1 or page_size < 1 or head_dim < 1 or head_dim % 8:
             raise ValueError("kv_heads, page_size and head_dim must be positive, head_dim a multiple of 8")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"a cache holds float16 or bfloat16, not {dtype}")
         device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         if device.type != "cuda":
             raise ValueError("the cache lives on a GPU")
@@ -48,7 +50,7 @@ class PagedKVCache:
         seqs, tokens = list(seqs), k.shape[1]
         if k.shape[0] != len(seqs) or (counts is not None and not all(0 <= c <= tokens for c in counts)):
             raise ValueError("one row of tokens for each sequence, and counts within them")
-        for x in (k, v):  # (all that could be refused, before the pool changes)
+        for x in (k, v):
             if x.shape != k.shape or x.shape[2:] != self.data.shape[2::2] or x.dtype != self.data.dtype or x.device != self.data.device:
                 raise ValueError("k and v must have the cache's heads, dtype and device")
             if x.requires_grad and torch.is_grad_enabled():
@@ -56,8 +58,12 @@ class PagedKVCache:
         starts = self.pool.lengths(seqs)
         new = [tokens] * len(seqs) if counts is None else [int(c) for c in counts]
         self.pool.grow(seqs, new)
-        table, starts, new = self._on_device(self.pool.table(seqs, 0), starts, torch.tensor(new, dtype=torch.int32))
-        cache_append(_rows(k), _rows(v), self.data, table, starts, None if counts is None else new)
+        try:
+            table, starts, stored = self._on_device(self.pool.table(seqs, 0), starts, torch.tensor(new, dtype=torch.int32))
+            cache_append(_rows(k), _rows(v), self.data, table, starts, None if counts is None else stored)
+        except BaseException:
+            self.pool.shrink(seqs, new)  # the sequences do not end in tokens that have not been stored
+            raise
 
     def attend(self, seqs: Sequence[int], q: torch.Tensor, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -68,8 +74,12 @@ class PagedKVCache:
     def fork(self, seq: int) -> int:
         """A new sequence with the tokens of another: full pages are shared, a last page that is not full is copied."""
         new, moves = self.pool.fork(seq)
-        if moves.shape[0]:
-            copy_pages(self.data, moves)
+        try:
+            if moves.shape[0]:
+                copy_pages(self.data, moves)
+        except BaseException:
+            self.pool.free(new)
+            raise
         return new
 
     def free(self, seq: int) -> None:
@@ -77,6 +87,7 @@ class PagedKVCache:
 
     def compact(self) -> int:
         """Moves the pages in use to the front; returns how many were moved.  Tables made before are no longer right."""
+        copy_pages(self.data, torch.empty((0, 2), dtype=torch.int32))  # (refused, if copying is, before the pool changes)
         moves = self.pool.compact()
         if moves.shape[0]:
             copy_pages(self.data, moves)

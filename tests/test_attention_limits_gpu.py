@@ -75,3 +75,33 @@ def test_small_weights_of_half_precision(dim):
             want = big * small / (large + small)
             tol = want * (2.0 ** -5.5 + 2.0 ** -10 + 2 * delta + n * 2.0 ** -23) + 2.0 ** -25
             assert (got[s].double() - want).abs().max() <= tol, (n, want, got[s])
+
+
+def test_what_a_cache_refuses_leaves_no_tokens_behind():
+    from flashoverlap_b200.models import PagedKVCache
+
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        PagedKVCache(4, 16, 2, 64, dtype=torch.float32)
+    cache = PagedKVCache(10, 16, 2, 64, dtype=BF16)
+    a, b = cache.add(), cache.add()
+    x = randn(2, 20, 2, 64, dtype=BF16)
+    cache.append([a, b], x, x)
+    before = [cache.length(s) for s in (a, b)], [cache.pool.pages(s) for s in (a, b)], cache.pool.free_pages(), cache.data.clone()
+    inside = cache.data[0, 0].transpose(0, 1)[None, :14]             # keys that lie in the cache itself
+    with pytest.raises(RuntimeError, match="share memory"):
+        cache.append([a], inside, inside)
+    cache.data.requires_grad_()
+    with pytest.raises(RuntimeError, match="gradient"):
+        cache.append([b, a], x, x)
+    cache.data.requires_grad_(False)
+    assert ([cache.length(s) for s in (a, b)], [cache.pool.pages(s) for s in (a, b)], cache.pool.free_pages()) == before[:3]
+    assert torch.equal(cache.data, before[3])
+    cache.append([b], x[1:], x[1:])                                    # the pages it would have had
+    assert cache.length(b) == 40 and cache.pool.free_pages() == before[2] - 1
+    cache.free(a)                                                      # pages in front are free now, copies are refused
+    pages = cache.pool.pages(b)
+    cache.data.requires_grad_()
+    for call in (cache.compact, lambda: cache.fork(b)):
+        with pytest.raises(RuntimeError, match="gradient"):
+            call()
+    assert cache.pool.pages(b) == pages and cache.pool.num_sequences() == 1 and cache.pool.free_pages() == 7
