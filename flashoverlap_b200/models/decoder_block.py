@@ -94,32 +94,54 @@ class TPDecoderBlock(nn.Module):
         residual stream [tokens, hidden].  Returns (next layer's QKV for all
         tokens [tokens, qkv_rows], new residual shard [tokens/world, hidden]).
         With a ``cache`` (PagedKVCache) the tokens' keys and values are stored as the first
-        of its sequences ``seqs``, which have none yet."""
+        of its sequences ``seqs``, which have none yet; a call that raises stores nothing."""
+        if cache is None:
+            return self._after(self._attention(self._project(h_norm), batch, seq), resid)
+        self._check_cached_heads()
+        if seqs is None:
+            raise ValueError("with a cache, forward needs the sequences that the prompts become")
+        if any(cache.length(s) for s in seqs):
+            raise ValueError("forward stores whole prompts: the sequences must be empty")
         qkv = self._project(h_norm)
-        if cache is not None:
-            if any(cache.length(s) for s in seqs):
-                raise ValueError("forward stores whole prompts: the sequences must be empty")
-            _, k, v = self._heads(qkv, batch, seq)
-            cache.append(seqs, k, v)
-        return self._after(self._attention(qkv, batch, seq), resid)
+        _, k, v = self._heads(qkv, batch, seq)
+        cache.append(seqs, k, v)
+        try:
+            return self._after(self._attention(qkv, batch, seq), resid)
+        except BaseException:
+            cache.take_back(seqs, [seq] * batch)
+            raise
 
     @torch.no_grad()
     def decode(self, h_norm, resid, cache, seqs):
         """One new token of each of the cache's sequences ``seqs``: h_norm and resid are [len(seqs), hidden].
         The token's key and value are stored, and it attends over all of its sequence.  Returns (next layer's QKV
-        [len(seqs), qkv_rows], new residual: this rank's share of the rows, which are padded to 128 a rank)."""
-        if self.head_dim not in (64, 128):
-            raise ValueError(f"attention over a cache takes heads of 64 or 128 values, not {self.head_dim}")
+        [len(seqs), qkv_rows], new residual: this rank's share of the rows, which are padded to 128 a rank).  A call
+        that raises stores nothing."""
+        self._check_cached_heads()
         n = len(seqs)
+        if h_norm.shape[0] != n or resid.shape[0] != n:
+            raise ValueError(f"one row for each of the {n} sequences, not {h_norm.shape[0]} and {resid.shape[0]}")
         pad = -n % (128 * self.world)
         h_norm, resid = (F.pad(x, (0, 0, 0, pad)) if pad else x for x in (h_norm, resid))
         qkv = self._project(h_norm)
         q, k, v = self._heads(qkv[:n], n, 1)
         cache.append(seqs, k, v)
-        attn = qkv.new_zeros((n + pad, self.heads * self.head_dim))
-        cache.attend(seqs, q[:, 0], window=self.window, sinks=self.sinks, out=attn[:n].view(n, self.heads, self.head_dim))
-        qkv_next, h3 = self._after(attn, resid)
+        try:
+            attn = qkv.new_zeros((n + pad, self.heads * self.head_dim))
+            cache.attend(seqs, q[:, 0], window=self.window, sinks=self.sinks, out=attn[:n].view(n, self.heads, self.head_dim))
+            qkv_next, h3 = self._after(attn, resid)
+        except BaseException:
+            cache.take_back(seqs, [1] * n)
+            raise
         return qkv_next[:n], h3
+
+    def _check_cached_heads(self):
+        """Heads that attention over a cache would refuse are refused before anything is computed or stored."""
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"attention over a cache takes heads of 64 or 128 values, not {self.head_dim}")
+        if self.heads % self.kv_heads or self.heads // self.kv_heads > 128:
+            raise ValueError(f"attention over a cache takes up to 128 query heads for each key and value head, not "
+                             f"{self.heads} on {self.kv_heads}")
 
     def _project(self, h_norm):
         qkv = torch.empty((h_norm.shape[0], self.w_qkv.shape[0]), dtype=h_norm.dtype, device=h_norm.device)

@@ -65,6 +65,11 @@ class PagedKVCache:
             self.pool.shrink(seqs, new)  # the sequences do not end in tokens that have not been stored
             raise
 
+    def take_back(self, seqs: Sequence[int], counts: Sequence[int]) -> None:
+        """Removes the last ``counts[i]`` tokens of sequence ``seqs[i]``.  Refused where a sequence would end inside a page
+        that it shares with a fork."""
+        self.pool.shrink(list(seqs), [int(c) for c in counts])
+
     def attend(self, seqs: Sequence[int], q: torch.Tensor, window: int = 0, sinks: int = 0, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of each sequence's last token, ``q[len(seqs), heads, head_dim]``, over its tokens."""

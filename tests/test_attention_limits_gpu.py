@@ -105,3 +105,38 @@ def test_what_a_cache_refuses_leaves_no_tokens_behind():
         with pytest.raises(RuntimeError, match="gradient"):
             call()
     assert cache.pool.pages(b) == pages and cache.pool.num_sequences() == 1 and cache.pool.free_pages() == 7
+
+
+def test_a_block_that_fails_leaves_no_tokens_behind():
+    # the products behind the attention refuse their shapes, or the attention itself does
+    from flashoverlap_b200.models import PagedKVCache
+    from flashoverlap_b200.models.decoder_block import TPDecoderBlock
+
+    block = TPDecoderBlock(None, 256, 64, 4, 2)
+    block._project = lambda h: h @ block.w_qkv.t()
+    cache = PagedKVCache(12, 16, 2, 64)
+    a, b = cache.add(), cache.add()
+    x = randn(1, 20, 2, 64, dtype=BF16)
+    cache.append([b], x, x)
+    h = randn(40, 256, dtype=BF16)
+
+    def refuse(*args, **kw):
+        raise RuntimeError("shape not supported")
+
+    def state():
+        return [cache.length(s) for s in (a, b)], [cache.pool.pages(s) for s in (a, b)], cache.pool.free_pages()
+
+    before = state()
+    block._after = refuse
+    for call in (lambda: block(h, h, 1, 40, cache=cache, seqs=[a]), lambda: block.decode(h[:2], h[:2], cache, [a, b])):
+        with pytest.raises(RuntimeError, match="not supported"):
+            call()
+        assert state() == before
+    block._attention = cache.attend = refuse
+    block._after = lambda attn, resid: (attn, resid)
+    for call in (lambda: block(h, h, 1, 40, cache=cache, seqs=[a]), lambda: block.decode(h[:2], h[:2], cache, [a, b])):
+        with pytest.raises(RuntimeError, match="not supported"):
+            call()
+        assert state() == before
+    cache.take_back([b], [5])
+    assert cache.length(b) == 15 and cache.pool.free_pages() == before[2] + 1
