@@ -22,13 +22,23 @@ void check_launch(cudaError_t e, const char* op) {
   TORCH_CHECK(e == cudaSuccess, op, " launch failed: ", cudaGetErrorString(e));
 }
 
+// There are no derivatives: neither a gradient nor a forward-mode tangent is dropped without a word.
+void check_no_derivative(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
+              " requires a gradient: these operators have no backward pass, call them under torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(0).defined(), name, " carries a forward-mode tangent: these operators have no derivative");
+}
+// A change that autograd is to know of.
+void count_change(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // [.., head_dim] rows on 16-byte boundaries.  A dimension of one entry may have any stride.
 void check_rows(const at::Tensor& t, const char* name, int64_t dims) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == dims, name, " must be ", dims, "-D, got ", t.dim(), "-D");
   dtype_of(t);
-  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), name,
-              " requires a gradient: these operators have no backward pass, call them under torch.no_grad()");
+  check_no_derivative(t, name);
   TORCH_CHECK(t.size(-1) <= 1 || t.stride(-1) == 1, name, ": the last dimension must be contiguous");
   for (int64_t d = 0; d + 1 < dims; ++d) {
     TORCH_CHECK(t.size(d) <= 1 || t.stride(d) % 8 == 0, name, ": strides must be multiples of 16 bytes");
@@ -215,6 +225,7 @@ static void prompt_attention_op(at::Tensor q, at::Tensor k, at::Tensor v, at::Te
     workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
     p.workspace = workspace.data_ptr();
   }
+  count_change(out);
   check_launch(launch_prompt_attention(p, dtype_of(q), at::cuda::getCurrentCUDAStream().stream()), "prompt_attention");
 }
 
@@ -271,6 +282,7 @@ static void paged_attention_op(at::Tensor q, at::Tensor cache, at::Tensor page_t
     workspace = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
     p.workspace = workspace.data_ptr();
   }
+  count_change(out);
   check_launch(launch_paged_attention(p, dtype_of(q), at::cuda::getCurrentCUDAStream().stream()), "paged_attention");
 }
 
@@ -320,6 +332,7 @@ static void cache_append_op(at::Tensor k, at::Tensor v, at::Tensor cache, at::Te
   p.tokens = static_cast<int>(tokens);
   p.width = static_cast<int>(page_table.size(1));
   c10::cuda::CUDAGuard guard(k.device());
+  count_change(cache);
   check_launch(launch_cache_append(p, at::cuda::getCurrentCUDAStream().stream()), "cache_append");
 }
 
@@ -354,8 +367,8 @@ static void copy_pages_op(at::Tensor cache, at::Tensor moves) {
   std::vector<int> list;
   if (moves.scalar_type() == at::kInt) read_moves<int>(moves, cache.size(0), list);
   else read_moves<int64_t>(moves, cache.size(0), list);
+  check_no_derivative(cache, "cache");
   TORCH_CHECK(cache.is_cuda(), "cache must be a CUDA tensor");
-  TORCH_CHECK(!(at::GradMode::is_enabled() && cache.requires_grad()), "cache requires a gradient");
   if (list.empty()) return;
   int64_t values = 1;
   for (int64_t d = cache.dim() - 1; d >= 1; --d) {
@@ -370,6 +383,7 @@ static void copy_pages_op(at::Tensor cache, at::Tensor moves) {
               "cache: pages must begin and end on 16-byte boundaries");
   TORCH_CHECK(bytes < (1ll << 33), "cache: a page holds too much");
   c10::cuda::CUDAGuard guard(cache.device());
+  count_change(cache);
   check_launch(launch_copy_pages(cache.data_ptr(), bytes, stride, list.data(), static_cast<int>(list.size() / 2),
                                  at::cuda::getCurrentCUDAStream().stream()),
                "copy_pages");
@@ -413,12 +427,18 @@ static std::vector<int64_t> seen_tiles_op(int64_t p0, int64_t p1, int64_t length
 }  // namespace fo
 
 TORCH_LIBRARY_FRAGMENT(flashoverlap_op, m) {
-  m.def("prompt_attention", &fo::prompt_attention_op);
-  m.def("prompt_attention_new", &fo::prompt_attention_new_op);
-  m.def("paged_attention", &fo::paged_attention_op);
-  m.def("paged_attention_new", &fo::paged_attention_new_op);
-  m.def("cache_append", &fo::cache_append_op);
-  m.def("copy_pages", &fo::copy_pages_op);
+  // (a!): what a call changes
+  m.def("prompt_attention(Tensor q, Tensor k, Tensor v, Tensor(a!) out, int window, int sinks, Tensor? lengths, float? scale)"
+        " -> ()", &fo::prompt_attention_op);
+  m.def("prompt_attention_new(Tensor q, Tensor k, Tensor v, int window, int sinks, Tensor? lengths, float? scale) -> Tensor",
+        &fo::prompt_attention_new_op);
+  m.def("paged_attention(Tensor q, Tensor cache, Tensor page_table, Tensor lengths, Tensor(a!) out, int window, int sinks,"
+        " float? scale) -> ()", &fo::paged_attention_op);
+  m.def("paged_attention_new(Tensor q, Tensor cache, Tensor page_table, Tensor lengths, int window, int sinks, float? scale)"
+        " -> Tensor", &fo::paged_attention_new_op);
+  m.def("cache_append(Tensor k, Tensor v, Tensor(a!) cache, Tensor page_table, Tensor starts, Tensor? counts) -> ()",
+        &fo::cache_append_op);
+  m.def("copy_pages(Tensor(a!) cache, Tensor moves) -> ()", &fo::copy_pages_op);
   m.def("attention_status", &fo::attention_status_op);
   m.def("attention_reset", &fo::attention_reset_op);
   m.def("attention_set_timeout_ns", &fo::attention_set_timeout_ns_op);

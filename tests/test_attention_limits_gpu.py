@@ -140,3 +140,43 @@ def test_a_block_that_fails_leaves_no_tokens_behind():
         assert state() == before
     cache.take_back([b], [5])
     assert cache.length(b) == 15 and cache.pool.free_pages() == before[2] + 1
+
+
+def test_tangents_are_refused_and_changes_are_counted():
+    import torch.autograd.forward_ad as fwAD
+
+    q, k = randn(2, 8, 4, 64, dtype=FP16), randn(2, 16, 2, 64, dtype=FP16)
+    cache = randn(6, 2, 2, 8, 64, dtype=FP16)
+    table, lens = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), ints(1, 1)
+    with fwAD.dual_level():
+        def dual(x):
+            return fwAD.make_dual(x, torch.ones_like(x))
+
+        for call in (lambda: ops.prompt_attention(dual(q), k, k), lambda: ops.prompt_attention(q, k, dual(k)),
+                     lambda: ops.paged_attention(dual(q[:, 0].contiguous()), cache, table, lens),
+                     lambda: ops.paged_attention(q[:, 0], dual(cache), table, lens),
+                     lambda: ops.cache_append(dual(k[:, :4].contiguous()), k[:, :4], cache, table, lens),
+                     lambda: ops.copy_pages(dual(cache), torch.tensor([[0, 1]]))):
+            with pytest.raises(RuntimeError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):   # tangents do not ask for gradients
+                call()
+    # what has been saved for a backward pass and is changed here is found out
+    for change in (lambda: ops.cache_append(k[:, :4], k[:, :4], cache, table, lens),
+                   lambda: ops.copy_pages(cache, torch.tensor([[0, 1]]))):
+        w = torch.ones(64, dtype=FP16, device="cuda", requires_grad=True)
+        y = (cache * w).sum()
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    out = torch.empty_like(q)
+    versions = out._version
+    ops.prompt_attention(q, k, k, out=out)
+    one = torch.empty_like(q[:, 0])
+    ops.paged_attention(q[:, 0], cache, table, lens, out=one)
+    assert out._version == versions + 1 and one._version == 1
+    with torch.inference_mode():                      # tensors that count nothing
+        inf = torch.zeros_like(cache)
+        ops.copy_pages(inf, torch.tensor([[0, 1]]))
+        ops.cache_append(k[:, :4], k[:, :4], inf, table, lens)
+    ops.copy_pages(inf, torch.tensor([[0, 1]]))
