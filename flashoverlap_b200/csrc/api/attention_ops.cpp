@@ -410,6 +410,17 @@ static std::vector<int64_t> page_place_op(std::vector<int64_t> row, int64_t pos,
   const int page = l.find(r.data(), static_cast<int>(r.size()), static_cast<int>(pos), place);
   return {page, place, page < 0 ? -1 : l.key_offset(page, static_cast<int>(head), place)};
 }
+// The tokens that position i sees in a sequence of `length` tokens, by the function the kernels use.
+static std::vector<int64_t> seen_tokens_op(int64_t i, int64_t length, int64_t window, int64_t sinks) {
+  TORCH_CHECK(i >= 0 && i < (1 << 20) && length >= 0 && length <= std::numeric_limits<int>::max(), "seen_tokens: bad arguments");
+  check_window(window, sinks);
+  std::vector<int64_t> out;
+  for (int64_t j = 0; j <= i + 1; ++j) {
+    if (is_visible(static_cast<int>(i), static_cast<int>(j), static_cast<int>(length), static_cast<int>(window),
+                   static_cast<int>(sinks))) out.push_back(j);
+  }
+  return out;
+}
 // First tokens of the tiles of `tile` tokens that the positions [p0, p1] of a sequence look at, by the function the kernels use.
 static std::vector<int64_t> seen_tiles_op(int64_t p0, int64_t p1, int64_t length, int64_t window, int64_t sinks, int64_t tile,
                                           int64_t align) {
@@ -443,5 +454,6 @@ TORCH_LIBRARY_FRAGMENT(flashoverlap_op, m) {
   m.def("attention_reset", &fo::attention_reset_op);
   m.def("attention_set_timeout_ns", &fo::attention_set_timeout_ns_op);
   m.def("page_place", &fo::page_place_op);
+  m.def("seen_tokens", &fo::seen_tokens_op);
   m.def("seen_tiles", &fo::seen_tiles_op);
 }

@@ -1,7 +1,7 @@
 // Attention over keys and values of a decoder: launch interface of the kernels (no PyTorch types), and the rules that the
 // kernels and the host share.
 //
-//   visible(i, j) = j <= i and (window == 0 or j > i - window or j < sinks) and j < length
+//   visible(i, j) = j <= i < length and (window == 0 or j > i - window or j < sinks)
 //   out_i = sum_j exp(scale q_i k_j) v_j / sum_j exp(scale q_i k_j) over the visible j, zero where there is none.
 //
 // A cache is [pages, 2, kv_heads, page_size, head_dim], keys at 0 and values at 1: what a page holds for one head is one
@@ -84,7 +84,7 @@ __host__ __device__ inline SeenTiles seen_tiles(int p0, int p1, int length, int 
   return t;
 }
 __host__ __device__ inline bool is_visible(int i, int j, int length, int window, int sinks) {
-  return j <= i && j < length && (window == 0 || i - j < window || j < sinks);
+  return j <= i && i < length && (window == 0 || i - j < window || j < sinks);
 }
 
 struct PromptParams {

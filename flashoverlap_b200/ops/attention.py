@@ -1,7 +1,7 @@
 """Attention of a decoder and its paged key-value cache, as functions of tensors.
 
-The token at position j is visible from position i if ``j <= i`` and (``window == 0`` or ``j > i - window`` or
-``j < sinks``) and j lies before the sequence's length.  Query head h reads key and value head
+The token at position j is visible from position i if ``j <= i < length`` (the sequence's length) and (``window == 0`` or
+``j > i - window`` or ``j < sinks``): positions behind the length see nothing.  Query head h reads key and value head
 ``h // (heads // kv_heads)``.  A row that sees nothing is zero.  float16 and bfloat16, head_dim 64 or 128; scores, sums and
 the statistics of the softmax are fp32, weights are rounded to the type of the values before they meet them.
 
