@@ -120,7 +120,8 @@ void check_table(const at::Tensor& table, int64_t seqs, const PageLayout& l, con
 }
 
 // What the prompt kernel reports of waits that ran out: a word for each device, in host memory that all devices see under
-// its own address, read before each call without waiting for anything.  Allocated at the first call, also where that is being captured, and kept.
+// its own address, read before each call without waiting for anything.  Allocated at the first call, also where that is
+// being captured, and kept.
 constexpr int kStatusDevices = 64;
 std::atomic<StatusWord*> status_words{nullptr};
 std::atomic<int64_t> prompt_wait_ns{10000000000};

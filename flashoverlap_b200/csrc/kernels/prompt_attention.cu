@@ -35,8 +35,8 @@
 // TMEM; 16 powers a clock and SM would be 1024), the products and the next scores 1000; the two groups of warps run half a
 // turn apart.  Long calls run at the power cap: 16384 tokens, 8 heads on 1, fp16, 494 to 506 us call after call (1.1 PFLOP/s,
 // 0.8 of cuBLAS's sustained bf16 rate), 445 in a short burst.  2 x 4096 tokens, 32 heads on 8, window 1024, bf16: 160 to 164 us
-// (the cap again; 145 in a short burst), ten tiles of keys for 8.3 that are seen, and 7000 clocks a pair for its first scores and its results.  3 x
-// 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 32 us; 77 tokens: 7.7 a call.
+// (the cap again; 145 in a short burst), ten tiles of keys for 8.3 that are seen, and 7000 clocks a pair for its first scores
+// and its results.  3 x 500 tokens behind 4503, 12 heads of 64 on 4, window 2048: 32 us; 77 tokens: 7.7 a call.
 //
 // Tried and slower: two threads a row (16 warps of softmax; 16384 tokens 588 us), results stored by TMA or row by row, the
 // second half of the scores read again after the first weights have left, tiles multiplied and weighed by quarters.  A lane
